@@ -32,6 +32,7 @@ from .ddp import DDP, DistributedDataParallel
 from .fsdp import FSDP, FullyShardedDataParallel, MixedPrecisionPolicy
 from .graphs import GraphedStep
 from .mesh import ParallelMesh
+from .ops.rotary import RotaryScaling, apply_rotary, rotary_table
 from .pipeline import PipelineStage, build_schedule, partition_layers, theoretical_bubble_fraction
 from .profiling import analyze_trace, format_collective_table, profile_steps, summarize_collectives
 from .tensor_parallel import (
@@ -58,6 +59,9 @@ __all__ = [
     "DistributedGradScaler",
     "PrecisionConfig",
     "vocab_parallel_cross_entropy",
+    "RotaryScaling",
+    "apply_rotary",
+    "rotary_table",
     "build_schedule",
     "partition_layers",
     "theoretical_bubble_fraction",

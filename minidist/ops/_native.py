@@ -12,6 +12,7 @@ GPU is known to have run the hand-written kernels.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -209,6 +210,14 @@ def check_status(device=None, reset: bool = True) -> None:
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return int(s.cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``t``'s device is current (free when it already is)."""
+    return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

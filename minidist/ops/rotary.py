@@ -1,0 +1,233 @@
+"""Rotary positions: cos / sin tables and their application to query and key heads.
+
+A pair ``(a, b)`` of channels of a token at position ``p`` turns by ``p * f_i``::
+
+    a' = a cos(p f_i) - b sin(p f_i)        f_i = base ** (-2 i / rotary_dim)
+    b' = b cos(p f_i) + a sin(p f_i)
+
+The first ``rotary_dim`` channels of each head turn, the others pass through.  On CUDA
+:func:`apply_rotary` is one sm_100a launch for queries and keys together
+(csrc/rotary.cu), on CPU the same arithmetic with torch operations; both
+differentiate (the gradient is the rotation back).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _native as nat
+
+__all__ = ["RotaryScaling", "rotary_table", "apply_rotary"]
+
+nat.declare("md_rotary", "i:pp")
+
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How frequencies are stretched for contexts ``factor`` times longer than trained.
+
+    ``kind``: ``"linear"`` divides every position by ``factor`` (position interpolation);
+    ``"ntk"`` raises the base to ``base * factor ** (r / (r - 2))``; ``"yarn"`` interpolates
+    per frequency, keeping those that turn more than ``beta_fast`` times over
+    ``original_positions``, dividing those that turn less than ``beta_slow`` times and blending
+    in between, and multiplies cos and sin by ``0.1 ln(factor) + 1``.
+    """
+
+    kind: str = "linear"
+    factor: float = 1.0
+    original_positions: int = 8192
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "yarn"):
+            raise ValueError(f"RotaryScaling kind {self.kind!r}: expected 'linear', 'ntk' or 'yarn'")
+        if not self.factor >= 1.0:
+            raise ValueError(f"RotaryScaling factor {self.factor}: expected a value of at least 1")
+
+
+def rotary_table(rotary_dim: int, positions: int, *, base: float = 10000.0, scaling: RotaryScaling | None = None,
+                 device=None) -> torch.Tensor:
+    """``[positions, rotary_dim / 2, 2]`` fp32 (cos, sin), computed in 64 bits and rounded once."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim={rotary_dim}: expected a positive even number")
+    if positions < 0 or not base > 0:
+        raise ValueError(f"positions={positions}, base={base}: expected non-negative and positive")
+    r, scale = rotary_dim, 1.0
+    pair = torch.arange(r // 2, dtype=torch.float64, device=device)
+    if scaling is not None and scaling.kind == "ntk" and r > 2:
+        base = base * scaling.factor ** (r / (r - 2))
+    freq = base ** (-2.0 * pair / r)
+    if scaling is not None and scaling.kind == "linear":
+        freq = freq / scaling.factor
+    elif scaling is not None and scaling.kind == "yarn":
+        def pair_turning(times: float) -> float:  # the pair that turns so often over the original context
+            return r * math.log(scaling.original_positions / (2 * math.pi * times)) / (2 * math.log(base))
+
+        lo = max(math.floor(pair_turning(scaling.beta_fast)), 0)
+        hi = min(math.ceil(pair_turning(scaling.beta_slow)), r - 1)
+        stretch = ((pair - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - stretch) + freq / scaling.factor * stretch
+        scale = 0.1 * math.log(scaling.factor) + 1.0
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return (torch.stack([angle.cos(), angle.sin()], dim=-1) * scale).float()
+
+
+class _Params(ctypes.Structure):
+    """Mirror of ``struct MdRotaryParams`` in csrc/rotary.cu."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p * 2),
+        ("y", ctypes.c_void_p * 2),
+        ("xs", (ctypes.c_longlong * 3) * 2),
+        ("ys", (ctypes.c_longlong * 3) * 2),
+        ("heads", ctypes.c_int * 2),
+        ("table", ctypes.c_void_p),
+        ("table_rows", ctypes.c_longlong),
+        ("positions", ctypes.c_void_p),
+        ("positions64", ctypes.c_int),
+        ("ps", ctypes.c_longlong * 2),
+        ("batch", ctypes.c_int),
+        ("seq", ctypes.c_int),
+        ("dim", ctypes.c_int),
+        ("rotary", ctypes.c_int),
+        ("interleaved", ctypes.c_int),
+        ("inverse", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+def _launch(q, k, q_out, k_out, table, positions, interleaved: bool, inverse: bool) -> None:
+    B, S, H, D = q.shape
+    p = _Params()
+    p.x[0], p.y[0] = q.data_ptr(), q_out.data_ptr()
+    p.xs[0][:] = q.stride()[:3]
+    p.ys[0][:] = q_out.stride()[:3]
+    p.heads[0] = H
+    if k is not None:
+        p.x[1], p.y[1] = k.data_ptr(), k_out.data_ptr()
+        p.xs[1][:] = k.stride()[:3]
+        p.ys[1][:] = k_out.stride()[:3]
+        p.heads[1] = k.shape[2]
+    p.table, p.table_rows = table.data_ptr(), table.shape[0]
+    if positions is not None:
+        p.positions, p.positions64 = positions.data_ptr(), positions.dtype == torch.int64
+        st = positions.stride()
+        p.ps[:] = (0, st[0]) if positions.dim() == 1 else st
+    p.batch, p.seq, p.dim, p.rotary = B, S, D, 2 * table.shape[1]
+    p.interleaved, p.inverse, p.dtype = interleaved, inverse, _DTYPE_CODE[q.dtype]
+    p.status = nat.status_ptr(q.device)
+    with nat.on_device(q):
+        nat.check(nat.lib().md_rotary(ctypes.addressof(p), nat.stream_ptr()), "md_rotary")
+
+
+def _turn_cpu(x, table, positions, interleaved, inverse):
+    cs = table[: x.shape[1]] if positions is None else table[positions.long()]
+    cos, sin = cs[..., 0].unsqueeze(-2), cs[..., 1].unsqueeze(-2)
+    if inverse:
+        sin = -sin
+    r = 2 * table.shape[1]
+    f = x.float()
+    a, b = (f[..., 0:r:2], f[..., 1:r:2]) if interleaved else (f[..., : r // 2], f[..., r // 2: r])
+    y = [a * cos - b * sin, b * cos + a * sin]
+    y = torch.stack(y, -1).flatten(-2) if interleaved else torch.cat(y, -1)
+    return torch.cat([y, f[..., r:]], -1).to(x.dtype)
+
+
+def _turn(q, k, table, positions, interleaved, inverse, inplace=False):
+    if not q.is_cuda:
+        out = [None if t is None else _turn_cpu(t, table, positions, interleaved, inverse) for t in (q, k)]
+        if not inplace:
+            return out
+        for t, o in zip((q, k), out):
+            if t is not None:
+                t.copy_(o)
+        return [q, k]
+    if inplace:
+        q_out, k_out = q, k
+    else:
+        q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (q, k))
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _launch(q, k, q_out, k_out, table, positions, interleaved, inverse)
+    return [q_out, k_out]
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, table, positions, interleaved, inverse):
+        ctx.save_for_backward(table, positions)
+        ctx.how = (interleaved, inverse)
+        ctx.set_materialize_grads(False)
+        return tuple(_turn(q, k, table, positions, interleaved, inverse))
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        table, positions = ctx.saved_tensors
+        interleaved, inverse = ctx.how
+        if dq is None and dk is None:
+            return (None,) * 6
+        if dq is None:
+            (dk, _) = _Rotary.apply(dk, None, table, positions, interleaved, not inverse)
+        else:
+            dq, dk = _Rotary.apply(dq, dk, table, positions, interleaved, not inverse)
+        return dq, dk, None, None, None, None
+
+
+def _check(q, k, table, positions) -> None:
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("apply_rotary expects q and k of [batch, seq, heads, head_dim]")
+    if q.dtype not in _DTYPE_CODE:
+        raise TypeError(f"apply_rotary: dtype {q.dtype} is not bfloat16, float16 or float32")
+    if k is not None and (k.dtype != q.dtype or k.device != q.device or k.shape[:2] != q.shape[:2]
+                          or k.shape[3] != q.shape[3]):
+        raise ValueError(f"apply_rotary: k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}")
+    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous() \
+            or table.device != q.device or not 0 < 2 * table.shape[1] <= q.shape[3]:
+        raise ValueError(f"apply_rotary: table {tuple(table.shape)} {table.dtype} is not a contiguous float32 "
+                         f"[positions, rotary_dim / 2, 2] on {q.device} with rotary_dim <= {q.shape[3]}")
+    if positions is None:
+        if q.shape[1] > table.shape[0]:
+            raise ValueError(f"apply_rotary: {q.shape[1]} tokens, but the table has {table.shape[0]} positions")
+    elif positions.dtype not in (torch.int64, torch.int32) or positions.device != q.device \
+            or tuple(positions.shape) not in ((q.shape[1],), tuple(q.shape[:2])):
+        raise ValueError(f"apply_rotary: positions {tuple(positions.shape)} {positions.dtype} are not int32 / int64 "
+                         f"[seq] or [batch, seq] on {q.device}")
+
+
+def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor | None = None,
+                 *, interleaved: bool = False):
+    """Queries ``[B, S, H, D]`` and keys ``[B, S, Hk, D]`` (or None) at their positions.
+
+    ``table``: from :func:`rotary_table`; its width says how many channels turn.  ``positions``:
+    int32 / int64 ``[S]`` or ``[B, S]``, by default 0, 1, .. S - 1.  ``interleaved`` pairs
+    neighbouring channels, otherwise a channel pairs with the one ``rotary_dim / 2`` further.
+    The inputs may be strided views (a packed QKV projection); the results are contiguous.  A
+    position outside the table makes its token's turned channels NaN and is reported by
+    :func:`minidist.ops._native.check_status` (on CPU it raises).
+    """
+    _check(q, k, table, positions)
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Rotary.apply(q, k, table, positions, interleaved, False)
+    return tuple(_turn(q, k, table, positions, interleaved, False))
+
+
+def rotate_packed_(qkv: torch.Tensor, heads: int, table: torch.Tensor, *, batch: int, inverse: bool = False):
+    """Turn the queries and keys of a packed ``[batch * seq, heads * (q, k, v) * dim]`` projection in
+    place (``inverse``: turn a packed gradient back).  No autograd: the fused block calls it in both
+    directions."""
+    rows, cols = qkv.shape
+    seq, dim = rows // batch, cols // (3 * heads)
+    view = qkv.as_strided((batch, seq, heads, 3, dim),
+                          (seq * qkv.stride(0), qkv.stride(0), 3 * dim, dim, 1), qkv.storage_offset())
+    q, k = view[:, :, :, 0], view[:, :, :, 1]
+    _check(q, k, table, None)
+    _turn(q, k, table, None, False, inverse, inplace=True)
+    return qkv

@@ -32,6 +32,7 @@ from .ddp import DDP, DistributedDataParallel
 from .fsdp import FSDP, FullyShardedDataParallel, MixedPrecisionPolicy
 from .graphs import GraphedStep
 from .mesh import ParallelMesh
+from .ops.logprobs import TokenLogprobs, token_logprobs
 from .ops.rotary import RotaryScaling, apply_rotary, rotary_table
 from .pipeline import PipelineStage, build_schedule, partition_layers, theoretical_bubble_fraction
 from .profiling import analyze_trace, format_collective_table, profile_steps, summarize_collectives
@@ -62,6 +63,8 @@ __all__ = [
     "RotaryScaling",
     "apply_rotary",
     "rotary_table",
+    "TokenLogprobs",
+    "token_logprobs",
     "build_schedule",
     "partition_layers",
     "theoretical_bubble_fraction",

@@ -33,6 +33,7 @@ from .fsdp import FSDP, FullyShardedDataParallel, MixedPrecisionPolicy
 from .graphs import GraphedStep
 from .mesh import ParallelMesh
 from .ops.logprobs import TokenLogprobs, token_logprobs
+from .ops.muon import orthogonalize
 from .ops.rotary import RotaryScaling, apply_rotary, rotary_table
 from .pipeline import PipelineStage, build_schedule, partition_layers, theoretical_bubble_fraction
 from .profiling import analyze_trace, format_collective_table, profile_steps, summarize_collectives
@@ -65,6 +66,7 @@ __all__ = [
     "rotary_table",
     "TokenLogprobs",
     "token_logprobs",
+    "orthogonalize",
     "build_schedule",
     "partition_layers",
     "theoretical_bubble_fraction",

@@ -1,0 +1,221 @@
+"""Orthogonalised updates: Newton-Schulz products and the Muon step around them.
+
+``X = U / (|U|_F + eps)``, then ``steps`` times (for the shorter side's Gram matrix)::
+
+    A = X X^T        X = a X + (b A + c A A) X
+
+drives every singular value of ``U`` towards one and leaves its singular vectors
+(Jordan et al. 2024).  :func:`orthogonalize` is that alone; :func:`muon_update_` adds momentum and
+the weights' update, for many matrices at once; :class:`minidist.optim.Muon` is the optimizer.
+
+On CUDA equally shaped matrices go through one chain of launches on the tensor cores
+(csrc/muon.cu): the momentum pass, the norm, three products a step, the last of which updates the
+weights in its epilogue.  On CPU the same arithmetic runs with torch operations.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from collections.abc import Sequence
+
+import torch
+
+from . import _native as nat
+
+__all__ = ["orthogonalize", "muon_update_", "COEFFICIENTS"]
+
+nat.declare("md_muon", "i:pp")
+nat.declare("md_muon_workspace", "l:iiii")
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_BATCH = 64
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class _Params(ctypes.Structure):
+    """Mirror of ``struct MdMuonParams`` in csrc/muon.cu."""
+
+    _fields_ = [
+        ("count", ctypes.c_int),
+        ("rows", ctypes.c_int),
+        ("cols", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+        ("step", ctypes.c_int),
+        ("split", ctypes.c_int),
+        ("iterations", ctypes.c_int),
+        ("a", ctypes.c_float),
+        ("b", ctypes.c_float),
+        ("c", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("momentum", ctypes.c_float),
+        ("nesterov", ctypes.c_int),
+        ("decay", ctypes.c_float),
+        ("rate", ctypes.c_float),
+        ("lr", ctypes.c_void_p),
+        ("inv_scale", ctypes.c_void_p),
+        ("skip", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_longlong),
+        ("tile", ctypes.c_int),
+        ("status", ctypes.c_void_p),
+        ("src", ctypes.c_void_p * _BATCH),
+        ("m", ctypes.c_void_p * _BATCH),
+        ("out", ctypes.c_void_p * _BATCH),
+        ("shadow", ctypes.c_void_p * _BATCH),
+    ]
+
+
+def _params(count, rows, cols, dtype, split, steps, coefficients, eps, device):
+    p = _Params()
+    p.count, p.rows, p.cols, p.dtype, p.split, p.iterations = count, rows, cols, dtype, split, steps
+    p.a, p.b, p.c = coefficients
+    p.eps = eps
+    size = nat.lib().md_muon_workspace(count, rows, cols, split)
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
+    p.workspace, p.workspace_bytes = workspace.data_ptr(), size
+    p.status = nat.status_ptr(device)
+    return p, workspace
+
+
+def _check_polynomial(steps, coefficients, eps) -> None:
+    if steps < 1 or len(coefficients) != 3 or not eps >= 0.0:
+        raise ValueError(f"Newton-Schulz: steps={steps}, coefficients={coefficients}, eps={eps}: expected at least one "
+                         "step, three coefficients and a non-negative eps")
+
+
+def _orthogonal_cpu(u: torch.Tensor, steps, coefficients, eps) -> torch.Tensor:
+    a, b, c = coefficients
+    x = u.float()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    for _ in range(steps):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    return x.mT if tall else x
+
+
+def _orthogonalize_cuda(u: torch.Tensor, steps, coefficients, eps, tile: int = 0) -> torch.Tensor:
+    rows, cols = u.shape[-2:]
+    u = u.contiguous()
+    out = torch.empty_like(u)
+    count = u.numel() // (rows * cols)
+    # A bf16 answer is rounded more coarsely than one product of fp16 parts errs; fp16 and fp32
+    # answers take the three-product form.
+    split = u.dtype != torch.bfloat16
+    size = rows * cols * u.element_size()
+    for at in range(0, count, _BATCH):
+        n = min(_BATCH, count - at)
+        p, workspace = _params(n, rows, cols, _DTYPE_CODE[u.dtype], split, steps, coefficients, eps, u.device)
+        p.tile = tile
+        src, dst = u.data_ptr() + at * size, out.data_ptr() + at * size
+        p.src[:n] = [src + i * size for i in range(n)]
+        p.out[:n] = [dst + i * size for i in range(n)]
+        with nat.on_device(u):
+            nat.check(nat.lib().md_muon(ctypes.addressof(p), nat.stream_ptr()), "md_muon")
+        del workspace  # (reused only by later work of this stream)
+    return out
+
+
+def orthogonalize(u: torch.Tensor, *, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """``u [..., rows, cols]`` (bfloat16, float16 or float32) with its singular values driven towards
+    one, each matrix by itself, in ``u``'s type.
+
+    The polynomial ``a s + b s^3 + c s^5`` has to keep ``|s| <= 1.3`` within about two, as the default
+    and the classical ``(1.5, -0.5, 0)`` and ``(15/8, -10/8, 3/8)`` do.  bfloat16 results are within a
+    bfloat16 rounding or so of exact, float16 and float32 ones within their own type's.  Not
+    differentiable."""
+    if u.dim() < 2 or u.dtype not in _DTYPE_CODE:
+        raise TypeError(f"orthogonalize: {tuple(u.shape)} {u.dtype} is not a bfloat16, float16 or float32 matrix")
+    _check_polynomial(steps, coefficients, eps)
+    u = u.detach()
+    if u.numel() == 0:
+        return u.clone()
+    if not u.is_cuda:
+        return _orthogonal_cpu(u, steps, coefficients, eps).to(u.dtype)
+    return _orthogonalize_cuda(u, steps, coefficients, eps)
+
+
+def _check_step(params, grads, momenta, shadows) -> None:
+    if not len(params) == len(grads) == len(momenta) or (shadows is not None and len(shadows) != len(params)):
+        raise ValueError("muon_update_: params, grads, momenta (and shadows) differ in number")
+    for i, (w, g, m) in enumerate(zip(params, grads, momenta)):
+        if w.dim() != 2 or w.dtype != torch.float32 or not w.is_contiguous():
+            raise ValueError(f"muon_update_: parameter {i} {tuple(w.shape)} {w.dtype} is not a contiguous float32 matrix")
+        if g.shape != w.shape or g.dtype != torch.float32 or g.device != w.device:
+            raise ValueError(f"muon_update_: gradient {i} {tuple(g.shape)} {g.dtype} does not go with {tuple(w.shape)}")
+        if m.shape != w.shape or m.dtype != torch.float32 or m.device != w.device or not m.is_contiguous():
+            raise ValueError(f"muon_update_: momentum {i} is not a contiguous float32 {tuple(w.shape)}")
+        sh = None if shadows is None else shadows[i]
+        if sh is not None and (sh.shape != w.shape or sh.dtype != torch.bfloat16 or sh.device != w.device
+                               or not sh.is_contiguous()):
+            raise ValueError(f"muon_update_: shadow {i} is not a contiguous bfloat16 {tuple(w.shape)}")
+
+
+def _scale(rows: int, cols: int, rms: float) -> float:
+    # An orthogonal [rows, cols] has entries of size 1 / sqrt(max(rows, cols)).
+    return rms * math.sqrt(max(rows, cols))
+
+
+@torch.no_grad()
+def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], *,
+                 lr: float | torch.Tensor, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+                 steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7, rms: float = 0.2,
+                 shadows: Sequence[torch.Tensor | None] | None = None, inv_scale: torch.Tensor | None = None,
+                 skip: torch.Tensor | None = None) -> None:
+    """One Muon step on fp32 matrices, in place::
+
+        m = momentum m + g        u = g + momentum m  (m without nesterov)
+        w = (1 - lr weight_decay) w - lr rms sqrt(max(rows, cols)) orthogonalize(u)
+
+    so that an update's entries have size ``lr rms`` whatever the shape (0.2 is AdamW's usual size,
+    whose learning rates then carry over).  ``lr`` may be a float32 tensor of one element on the
+    device.  ``shadows``: bfloat16 copies to refresh with the weights.  ``inv_scale`` / ``skip``: the
+    loss scaler's device factor on the gradients and its flag that leaves everything unchanged.
+    Matrices of one shape and device are updated together, 64 at a time."""
+    _check_polynomial(steps, coefficients, eps)
+    _check_step(params, grads, momenta, shadows)
+    groups: dict = {}
+    for i, w in enumerate(params):
+        groups.setdefault((w.shape, w.device), []).append(i)
+    for (shape, device), members in groups.items():
+        rows, cols = shape
+        if rows * cols == 0:
+            continue
+        if device.type != "cuda":
+            if skip is not None and bool(skip.item()):
+                continue
+            for i in members:
+                g = grads[i] if inv_scale is None else grads[i] * inv_scale
+                momenta[i].mul_(momentum).add_(g)
+                u = g.add(momenta[i], alpha=momentum) if nesterov else momenta[i]
+                x = _orthogonal_cpu(u, steps, coefficients, eps)
+                params[i].mul_(1 - lr * weight_decay).sub_(x * (lr * _scale(rows, cols, rms)))
+                if shadows is not None and shadows[i] is not None:
+                    shadows[i].copy_(params[i])
+            continue
+        for at in range(0, len(members), _BATCH):
+            part = members[at: at + _BATCH]
+            n = len(part)
+            # One product of fp16 parts: X errs by 1e-3 of itself, and the weights take lr rms of it.
+            p, workspace = _params(n, rows, cols, 2, False, steps, coefficients, eps, device)
+            p.step, p.momentum, p.nesterov = 1, momentum, nesterov
+            factor = _scale(rows, cols, rms)
+            if isinstance(lr, torch.Tensor):
+                if lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != device:
+                    raise ValueError(f"muon_update_: lr is not one float32 on {device}")
+                p.lr, p.decay, p.rate = lr.data_ptr(), weight_decay, factor
+            else:
+                p.decay, p.rate = 1.0 - lr * weight_decay, lr * factor
+            p.inv_scale, p.skip = nat.ptr(inv_scale), nat.ptr(skip)
+            held = [grads[i].contiguous() for i in part]
+            p.src[:n] = [g.data_ptr() for g in held]
+            p.m[:n] = [momenta[i].data_ptr() for i in part]
+            p.out[:n] = [params[i].data_ptr() for i in part]
+            if shadows is not None:
+                p.shadow[:n] = [nat.ptr(shadows[i]) for i in part]
+            with nat.on_device(params[part[0]]):
+                nat.check(nat.lib().md_muon(ctypes.addressof(p), nat.stream_ptr()), "md_muon")
+            del workspace, held  # (reused only by later work of this stream)

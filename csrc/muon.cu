@@ -66,7 +66,7 @@ namespace md {
 namespace muon {
 
 constexpr float kScale = 4096.f;  // fp16 operands hold kScale times the value
-constexpr int kChunk = 16384;     // elements per block of the norm and conversion passes
+constexpr int kChunk = 8192;      // elements per block of the norm and conversion passes
 constexpr int kThreads = 256;
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
@@ -158,7 +158,14 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
   const T* g = static_cast<const T*>(p.src[blockIdx.y]);
   const float* m = p.m[blockIdx.y];
   const float gs = STEP && p.inv_scale != nullptr ? *p.inv_scale : 1.f;
-  const long long base = static_cast<long long>(blockIdx.y) * p.rows * ldx;
+  // Position of the chunk's first element; inside the chunk 32-bit division is enough.
+  const long long row_lo = lo / p.cols;
+  const uint32_t col_lo = static_cast<uint32_t>(lo - row_lo * p.cols), cols = static_cast<uint32_t>(p.cols);
+  const long long base = (static_cast<long long>(blockIdx.y) * p.rows + row_lo) * ldx;
+  auto place = [&](uint32_t i) {  // of element lo + i
+    const uint32_t e = col_lo + i, r = e / cols;
+    return base + static_cast<long long>(r) * ldx + (e - r * cols);
+  };
   auto value = [&](float gv, float mv) {
     if (!STEP) return gv * inv;
     return (p.nesterov ? fmaf(p.momentum, mv, gv * gs) : mv) * inv;
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
     const Four<T> gv = *reinterpret_cast<const Four<T>*>(g + k);
     Four<float> mv = {};
     if (STEP) mv = *reinterpret_cast<const Four<float>*>(m + k);
-    const long long r = k / p.cols, o = base + r * ldx + (k - r * p.cols);
+    const long long o = place(static_cast<uint32_t>(4 * i));
     Four<__half> h, l;
 #pragma unroll
     for (int q = 0; q < 4; ++q) split_half(value(to_f(gv.v[q]), mv.v[q]), h.v[q], l.v[q]);
@@ -180,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
     *reinterpret_cast<Four<__half>*>(xl + o) = l;
   }
   for (long long k = lo + 4 * nv + threadIdx.x; k < hi; k += kThreads) {
-    const long long r = k / p.cols, o = base + r * ldx + (k - r * p.cols);
+    const long long o = place(static_cast<uint32_t>(k - lo));
     split_half(value(to_f(g[k]), STEP ? m[k] : 0.f), xh[o], xl[o]);
   }
 }
@@ -191,9 +198,11 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
 constexpr int BM = 128;   // rows of A and of B per CTA and stage
 constexpr int BK = 64;
 constexpr int kOperand = BM * BK * 2;  // 16 KB
-constexpr int kStages = 6;
+constexpr int kStages = 5;
 constexpr int kEpiWarps = 8;
-constexpr int kSmemBytes = 1024 + kStages * 2 * kOperand + 256;
+constexpr int kChunkBytes = 32 * 32 * 2;       // an epilogue chunk of fp16: 32 rows x 64 bytes
+constexpr int kWarpBytes = 4 * kChunkBytes;    // a warp's staging
+constexpr int kSmemBytes = 1024 + kStages * 2 * kOperand + kEpiWarps * kWarpBytes + 512;
 constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
 
 // Split products: the tensor core truncates as it accumulates, which over a long K costs a few bits of
@@ -207,9 +216,6 @@ struct GemmParams {
   int M, N, K;
   int tiles_m, tiles_n, per_batch, units, k_blocks;
   float alpha, beta;
-  const __half* c[2];       // kPoly: A, kNext / kLast: X (high, low or null)
-  __half* d[2];             // high, low or null
-  long long ldc, ldd, batch_c, batch_d;
   // kLast: what leaves
   int dtype, step;
   float decay, rate;
@@ -301,6 +307,20 @@ __device__ __forceinline__ void commit_own(uint64_t* bar) {
   }
 }
 
+// An epilogue chunk in and out (shared-memory addresses).
+__device__ __forceinline__ void tma_load_3d_at(const CUtensorMap* map, uint64_t* bar, uint32_t dst, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d_at(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 // Unit -> (matrix, tile row, tile column).  The symmetric products enumerate the tiles on and below
 // the diagonal only.
 template <bool SYM>
@@ -318,154 +338,138 @@ __device__ __forceinline__ void decode(const GemmParams& p, int u, int& b, int& 
   }
 }
 
-__device__ __forceinline__ void load32(const __half* src, bool full, int left, float (&f)[32]) {
-  if (full) {
+// Byte offset of a 16-byte piece in a chunk of 64-byte rows under the 64-byte TMA swizzle.
+__device__ __forceinline__ uint32_t sw64_off(int row, int piece) {
+  return static_cast<uint32_t>(row * 64 + ((piece ^ ((row >> 1) & 3)) << 4));
+}
+
+// f += the lane's row of a staged fp16 chunk times `by`.
+__device__ __forceinline__ void add_staged(uint32_t chunk, int lane, float by, float (&f)[32]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * q);
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  for (int q = 0; q < 4; ++q) {
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(chunk + sw64_off(lane, q)));
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&ws[k]));
-        f[8 * q + 2 * k] = v.x;
-        f[8 * q + 2 * k + 1] = v.y;
-      }
+    for (int k = 0; k < 4; ++k) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      f[8 * q + 2 * k] = fmaf(by, v.x, f[8 * q + 2 * k]);
+      f[8 * q + 2 * k + 1] = fmaf(by, v.y, f[8 * q + 2 * k + 1]);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = j < left ? __half2float(src[j]) : 0.f;
   }
 }
 
-// One accumulator row of a thread, 32 columns from n0: the epilogue of one chunk.  `acc` is in TMEM
-// (its load is issued here, ahead of C's) or, with split products, already in registers.
-template <int MODE, bool SPLIT>
-__device__ __forceinline__ void epilogue_chunk(const GemmParams& p, int b, int row0, int lane, int n0, uint32_t taddr,
-                                               const float* sum) {
-  const int row = row0 + lane;
-  const bool row_ok = row < p.M;
-  const bool full = n0 + 32 <= p.N;
-  const int left = p.N - n0;
-  constexpr bool SYM = MODE == kGram || MODE == kPoly;
-  if (SYM && n0 > row0 + 31) return;  // above the diagonal (warp-uniform)
-  uint32_t r[32];
-  if constexpr (!SPLIT) tmem_ld_32x32b_x32(taddr, r);
-  float cf[32], cl[32];
-  constexpr bool has_low = SPLIT || MODE == kNext || MODE == kLast;  // X is always a pair, A with split products
-  if (MODE != kGram && row_ok) {
-    const long long o = b * p.batch_c + row * p.ldc + n0;
-    load32(p.c[0] + o, full, left, cf);
-    if (has_low) load32(p.c[1] + o, full, left, cl);
-  }
-  if constexpr (!SPLIT) tmem_ld_wait();
-  if (!row_ok) return;  // (nothing warp-collective below)
-  float v[32];
+// The lane's row of a chunk, packed in pairs.
+__device__ __forceinline__ void stage(uint32_t chunk, int lane, const uint32_t (&w)[16]) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    v[j] = (SPLIT ? sum[j] : __uint_as_float(r[j])) * p.alpha;
-    if (MODE != kGram) v[j] = fmaf(p.beta, has_low ? cf[j] + cl[j] : cf[j], v[j]);
-  }
-  if constexpr (MODE == kLast) {
-    if (p.step) {
-      if (p.skip != nullptr && *p.skip != 0.f) return;
-      const float lr = p.lr != nullptr ? *p.lr : 1.f;
-      const float rate = p.rate * lr * (1.f / kScale), decay = p.lr != nullptr ? 1.f - lr * p.decay : p.decay;
-      float* w = static_cast<float*>(p.out[b]) + static_cast<long long>(row) * p.N + n0;
-      __nv_bfloat16* sh = p.shadow[b];
-      if (sh != nullptr) sh += static_cast<long long>(row) * p.N + n0;
-      if (full && (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && (reinterpret_cast<uintptr_t>(sh) & 7u) == 0) {
+  for (int q = 0; q < 4; ++q)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk + sw64_off(lane, q)), "r"(w[4 * q]),
+                 "r"(w[4 * q + 1]), "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                 : "memory");
+}
+// ... and its transpose: the lane's row becomes a column.
+__device__ __forceinline__ void stage_mirrored(uint32_t chunk, int lane, const uint32_t (&w)[16]) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          float4 t = *reinterpret_cast<const float4*>(w + 4 * q);
-          t.x = fmaf(t.x, decay, -rate * v[4 * q]);
-          t.y = fmaf(t.y, decay, -rate * v[4 * q + 1]);
-          t.z = fmaf(t.z, decay, -rate * v[4 * q + 2]);
-          t.w = fmaf(t.w, decay, -rate * v[4 * q + 3]);
-          *reinterpret_cast<float4*>(w + 4 * q) = t;
-          if (sh != nullptr) *reinterpret_cast<uint2*>(sh + 4 * q) = make_uint2(pack_bf16x2(t.x, t.y), pack_bf16x2(t.z, t.w));
-        }
+  for (int j = 0; j < 32; ++j)
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(chunk + sw64_off(j, lane >> 3) + (lane & 7) * 2),
+                 "h"(static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2]))
+                 : "memory");
+}
+
+// High and low fp16 parts of 32 values, packed in pairs (low parts only if asked for).
+template <bool LOW>
+__device__ __forceinline__ void split32(const float (&v)[32], uint32_t (&h)[16], uint32_t (&l)[16]) {
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const __half2 a = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
+    h[q] = *reinterpret_cast<const uint32_t*>(&a);
+    if (LOW) {
+      const float2 b = __half22float2(a);
+      const __half2 c = __floats2half2_rn(v[2 * q] - b.x, v[2 * q + 1] - b.y);
+      l[q] = *reinterpret_cast<const uint32_t*>(&c);
+    }
+  }
+}
+
+// What leaves: 32 x 32 fp32 values (kScale times X) staged in 128-byte rows, 16-byte pieces swizzled
+// by the row.  A lane takes four neighbouring columns of every fourth row, so that a warp's access is
+// four whole 128-byte lines; the weights to update are asked for one chunk ahead (`old`), because the
+// products' operand loads keep the L2 busy and a load issued at its use waits 3000 cycles.
+struct Out {
+  float rate, decay;
+  bool idle, wide;  // nothing to write; rows and addresses allow whole pieces
+};
+__device__ __forceinline__ void load_old(const GemmParams& p, const Out& o, int b, int row0, int n0, int lane, float4 (&old)[8]) {
+  const int col = n0 + (lane & 7) * 4;
+  if (!p.step || !o.wide || o.idle || col >= p.N) return;
+  const float* w = static_cast<const float*>(p.out[b]) + static_cast<long long>(row0 + (lane >> 3)) * p.N + col;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (row0 + 4 * i + (lane >> 3) < p.M) old[i] = *reinterpret_cast<const float4*>(w + 4ll * i * p.N);
+}
+__device__ __forceinline__ void write_out(const GemmParams& p, const Out& o, uint32_t staged, int b, int row0, int n0,
+                                          int lane, const float4 (&old)[8]) {
+  if (o.idle) return;
+  const int col = n0 + (lane & 7) * 4;
+  const int left = min(4, p.N - col);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    if (row0 + r >= p.M || left <= 0) continue;
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(staged + r * 128 + (((lane & 7) ^ (r & 7)) << 4)));
+    const long long at = static_cast<long long>(row0 + r) * p.N + col;
+    if (o.wide) {
+      if (p.step) {
+        v.x = fmaf(old[i].x, o.decay, o.rate * v.x), v.y = fmaf(old[i].y, o.decay, o.rate * v.y);
+        v.z = fmaf(old[i].z, o.decay, o.rate * v.z), v.w = fmaf(old[i].w, o.decay, o.rate * v.w);
       } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j < left) {
-            const float t = fmaf(w[j], decay, -rate * v[j]);
-            w[j] = t;
-            if (sh != nullptr) sh[j] = __float2bfloat16_rn(t);
-          }
+        v.x *= o.rate, v.y *= o.rate, v.z *= o.rate, v.w *= o.rate;
+      }
+      if (p.dtype == 2) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out[b]) + at) = v;
+        if (p.shadow[b] != nullptr)
+          *reinterpret_cast<uint2*>(p.shadow[b] + at) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+      } else if (p.dtype == 0) {
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out[b]) + at) =
+            make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+      } else {
+        const __half2 x = __floats2half2_rn(v.x, v.y), y = __floats2half2_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(static_cast<__half*>(p.out[b]) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
       }
     } else {
+      const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= 1.f / kScale;
-      const long long o = static_cast<long long>(row) * p.N + n0;
-      if (p.dtype == 2) {
-        float* w = static_cast<float*>(p.out[b]) + o;
-        if (full && (reinterpret_cast<uintptr_t>(w) & 15u) == 0) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(w + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      for (int j = 0; j < 4; ++j) {
+        if (j >= left) break;
+        if (p.step) {
+          float* w = static_cast<float*>(p.out[b]) + at + j;
+          const float t = fmaf(*w, o.decay, o.rate * f[j]);
+          *w = t;
+          if (p.shadow[b] != nullptr) p.shadow[b][at + j] = __float2bfloat16_rn(t);
+        } else if (p.dtype == 0) {
+          static_cast<__nv_bfloat16*>(p.out[b])[at + j] = __float2bfloat16_rn(f[j] * o.rate);
+        } else if (p.dtype == 1) {
+          static_cast<__half*>(p.out[b])[at + j] = __float2half_rn(f[j] * o.rate);
         } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < left) w[j] = v[j];
+          static_cast<float*>(p.out[b])[at + j] = f[j] * o.rate;
         }
-      } else {
-        uint32_t pk[16];
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          if (p.dtype == 0) {
-            pk[q] = pack_bf16x2(v[2 * q], v[2 * q + 1]);
-          } else {
-            const __half2 h = __floats2half2_rn(v[2 * q], v[2 * q + 1]);
-            pk[q] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        }
-        uint16_t* w = static_cast<uint16_t*>(p.out[b]) + o;
-        if (full && (reinterpret_cast<uintptr_t>(w) & 15u) == 0) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<uint4*>(w + 8 * q) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < left) w[j] = static_cast<uint16_t>(j & 1 ? pk[j / 2] >> 16 : pk[j / 2]);
-        }
-      }
-    }
-    return;
-  } else {
-    __align__(16) __half h[32];
-    __align__(16) __half l[32];
-#pragma unroll
-    for (int j = 0; j < 32; ++j) split_half(v[j], h[j], l[j]);
-    const bool below = !SYM || n0 + 31 <= row0;  // warp-uniform: no column above the diagonal
-#pragma unroll
-    for (int w = 0; w < (SPLIT || MODE == kNext ? 2 : 1); ++w) {
-      __half* d = p.d[w] + b * p.batch_d;
-      const __half* x = w == 0 ? h : l;
-      __half* dst = d + row * p.ldd + n0;
-      if (below && full) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(dst + 8 * q) = *reinterpret_cast<const uint4*>(x + 8 * q);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j < left && (!SYM || n0 + j <= row)) dst[j] = x[j];
-      }
-      if (SYM) {  // the mirrored half: 32 lanes write 32 neighbours of a row
-        __half* t = d + static_cast<long long>(n0) * p.ldd + row;
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j < left && (below || n0 + j < row)) t[j * p.ldd] = x[j];
       }
     }
   }
 }
+
+struct Maps {
+  CUtensorMap a[2], b[2], c[2], d[2];  // high and low parts: operands, addend, result
+};
 
 template <int CG, bool SPLIT, bool A_MN, bool B_MN, int MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    product_kernel(const __grid_constant__ CUtensorMap ah, const __grid_constant__ CUtensorMap al,
-                   const __grid_constant__ CUtensorMap bh, const __grid_constant__ CUtensorMap bl,
-                   const __grid_constant__ GemmParams p) {
+    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmParams p) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
   constexpr int BN = BM * CG;  // tile columns (and rows of the pair's tile)
   constexpr int kTmemCols = 2 * BN;
@@ -473,7 +477,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + kStages * kOperand;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 2 * kStages * kOperand);
+  uint8_t* sEpi = smem + 2 * kStages * kOperand;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + kEpiWarps * kWarpBytes);
   uint64_t* full_bar = bars;
   uint64_t* empty_bar = bars + kStages;
   uint64_t* tfull_bar = bars + 2 * kStages;
@@ -481,6 +486,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint64_t* drain_bar = bars + 2 * kStages + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * kStages + 6);
+  uint64_t* c_bar = bars + 2 * kStages + 7;  // two per epilogue warp
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = CG == 2 ? cluster_ctarank() : 0u;
@@ -498,10 +504,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       mbar_init(&tempty_bar[a], CG * kEpiWarps);
     }
     mbar_init(drain_bar, 1);
+    for (int i = 0; i < 2 * kEpiWarps; ++i) mbar_init(&c_bar[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&ah);
-    tma_prefetch_desc(&bh);
+    tma_prefetch_desc(&maps.a[0]);
+    tma_prefetch_desc(&maps.b[0]);
   }
   if (warp == 1) {
     if constexpr (CG == 2) {
@@ -538,8 +545,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int i = 0; i < blocks; ++i) {
         // high x high, high x low, low x high
         const int which = i / p.k_blocks, k = (i - which * p.k_blocks) * BK;
-        const CUtensorMap* ta = which == 2 ? &al : &ah;
-        const CUtensorMap* tb = which == 1 ? &bl : &bh;
+        const CUtensorMap* ta = &maps.a[which == 2];
+        const CUtensorMap* tb = &maps.b[which == 1];
         if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, 420, abort_flag)) {
           ok = false;
           break;
@@ -645,19 +652,62 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         acc_phase ^= 1u;
       }
     };
+    // Staging: slot = the addend's chunk (high, low) on arrival, the result's on departure.  Two slots,
+    // so that the next addend arrives under this chunk's arithmetic; one where a result with its
+    // mirror image needs both.
+    constexpr bool kAddend = MODE != kGram;
+    constexpr bool kAddLow = SPLIT || MODE == kNext || MODE == kLast;  // X is always a pair, A with split products
+    constexpr bool kLow = SPLIT || MODE == kNext;                      // the result is a pair
+    constexpr int kSlots = SPLIT && SYM ? 1 : 2;
+    const uint32_t base = smem_u32(sEpi) + (warp - 2) * kWarpBytes;
+    uint64_t* cb = c_bar + (warp - 2) * 2;
+    int ctr = 0;           // chunks done
+    int coming = 0;        // addends on their way, into the slots from ctr on
+    // Slot `i` may be overwritten: its own accesses are done (fence, warp barrier), its result has been read.
+    auto acquire = [&]() {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+    };
+    auto fetch = [&](int i, int b, int row0, int n0) {
+      acquire();
+      ++coming;
+      if (lane == 0) {
+        uint64_t* bar = &cb[i % kSlots];
+        const uint32_t dst = base + (i % kSlots) * (kWarpBytes / 2);
+        mbar_arrive_expect_tx(bar, kAddLow ? 2 * kChunkBytes : kChunkBytes);
+        tma_load_3d_at(&maps.c[0], bar, dst, n0, row0, b);
+        if (kAddLow) tma_load_3d_at(&maps.c[1], bar, dst + kChunkBytes, n0, row0, b);
+      }
+    };
     bool ok = true;
     for (int u = first; u < p.units && ok; u += stride) {
       int b, tm, tn;
       decode<SYM>(p, u, b, tm, tn);
       const int row0 = tm * (CG * BM) + static_cast<int>(crank) * BM + quarter * 32;
-      auto t_row = [&]() {
-        return tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
-      };
+      const int col0 = tn * BN + half * kChunks * 32;
+      // This warp's chunks: up to the last column, or the one that holds the diagonal.
+      const int end = SYM ? min(p.N, row0 + 32) : p.N;
+      const int chunks = row0 < p.M && end > col0 ? min(kChunks, (end - col0 + 31) / 32) : 0;
+      if (kAddend && chunks > 0) fetch(ctr, b, row0, col0);
+      Out out;
+      float4 old[8];
+      if constexpr (MODE == kLast) {
+        const float lr = p.lr != nullptr ? *p.lr : 1.f;
+        out.rate = p.step ? -p.rate * lr * (1.f / kScale) : 1.f / kScale;
+        out.decay = p.lr != nullptr ? 1.f - lr * p.decay : p.decay;
+        out.idle = p.step && p.skip != nullptr && *p.skip != 0.f;
+        const unsigned long long piece = p.dtype == 2 ? 15u : 7u;
+        out.wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out[b]) & piece) == 0 &&
+                   (reinterpret_cast<uintptr_t>(p.shadow[b]) & 7u) == 0;
+        if (chunks > 0) load_old(p, out, b, row0, col0, lane, old);
+      }
       float sum[SPLIT ? kChunks * 32 : 1];
       if constexpr (SPLIT) {
 #pragma unroll
         for (int j = 0; j < kChunks * 32; ++j) sum[j] = 0.f;
-        for (int i0 = 0; i0 < blocks; i0 += run) {
+        for (int i0 = 0; i0 < blocks && ok; i0 += run) {
           if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) {
             ok = false;
             break;
@@ -666,7 +716,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             uint32_t r[32];
-            tmem_ld_32x32b_x32(t_row() + (half * kChunks + c) * 32, r);
+            tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                   static_cast<uint32_t>(acc * BN + (half * kChunks + c) * 32), r);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) sum[c * 32 + j] += __uint_as_float(r[j]);
@@ -678,16 +729,88 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) break;
         tc_fence_after();
       }
-#pragma unroll(SPLIT ? kChunks : 1)
-      for (int c = 0; c < kChunks; ++c) {
-        const int n0 = tn * BN + (half * kChunks + c) * 32;
-        if (n0 >= p.N || row0 >= p.M) break;  // warp-uniform
-        epilogue_chunk<MODE, SPLIT>(p, b, row0, lane, n0, SPLIT ? 0u : t_row() + (half * kChunks + c) * 32,
-                                    SPLIT ? sum + c * 32 : nullptr);
-        __syncwarp();
+      auto chunk = [&](int c) {
+        const int n0 = col0 + c * 32;
+        const uint32_t slot = base + (ctr % kSlots) * (kWarpBytes / 2);
+        float v[32];
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j] * p.alpha;
+        } else {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                                 static_cast<uint32_t>(acc * BN + (half * kChunks + c) * 32), r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * p.alpha;
+        }
+        if constexpr (kAddend) {
+          if (kSlots == 2 && c + 1 < chunks) fetch(ctr + 1, b, row0, n0 + 32);
+          if (!mbar_wait(&cb[ctr % kSlots], static_cast<uint32_t>(ctr / kSlots) & 1u, p.status, 426, abort_flag)) {
+            ok = false;
+            return;
+          }
+          add_staged(slot, lane, p.beta, v);
+          if (kAddLow) add_staged(slot + kChunkBytes, lane, p.beta, v);
+          --coming;
+          __syncwarp();  // the whole chunk has been read
+        } else {
+          // (the other slot's result may still be leaving; this one's has to be out)
+          if (lane == 0) {
+            if (kSlots == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            else bulk_wait_read_all();
+          }
+          __syncwarp();
+        }
+        if constexpr (MODE == kLast) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(slot + lane * 128 + ((q ^ (lane & 7)) << 4)),
+                         "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
+                         : "memory");
+          __syncwarp();
+          write_out(p, out, slot, b, row0, n0, lane, old);
+          if (c + 1 < chunks) load_old(p, out, b, row0, n0 + 32, lane, old);
+        } else {
+          const bool mirrored = SYM && n0 < row0;  // (the block on the diagonal is its own mirror image)
+          uint32_t h[16], l[16];
+          split32<kLow>(v, h, l);
+          stage(slot, lane, h);
+          if (kLow) stage(slot + kChunkBytes, lane, l);
+          constexpr uint32_t kMirror = kLow ? 2 * kChunkBytes : kChunkBytes;
+          if (SYM && mirrored) {
+            stage_mirrored(slot + kMirror, lane, h);
+            if (kLow) stage_mirrored(slot + kMirror + kChunkBytes, lane, l);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d_at(&maps.d[0], slot, n0, row0, b);
+            if (kLow) tma_store_3d_at(&maps.d[1], slot + kChunkBytes, n0, row0, b);
+            if (SYM && mirrored) {
+              tma_store_3d_at(&maps.d[0], slot + kMirror, row0, n0, b);
+              if (kLow) tma_store_3d_at(&maps.d[1], slot + kMirror + kChunkBytes, row0, n0, b);
+            }
+            bulk_commit_group();
+          }
+        }
+        ++ctr;
+        if (kAddend && kSlots == 1 && c + 1 < chunks) fetch(ctr, b, row0, n0 + 32);
+      };
+      if constexpr (SPLIT) {  // (unrolled, so that the sums stay in registers)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          if (c < chunks && ok) chunk(c);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < chunks && ok; ++c) chunk(c);
       }
       if constexpr (!SPLIT) release();
     }
+    // Nothing may be in flight into or out of shared memory at exit.
+    for (; coming > 0; --coming, ++ctr)
+      mbar_wait(&cb[ctr % kSlots], static_cast<uint32_t>(ctr / kSlots) & 1u, p.status, 427, nullptr);
+    if (lane == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -717,28 +840,30 @@ bool get_encoder() {
   return true;
 }
 
-// A stack of fp16 matrices and its two tensor maps: 64 columns x 128 rows (K-major operand) and
-// 64 columns x 64 rows (MN-major).  Columns past the matrix read as zero.
+// A stack of fp16 matrices and its tensor maps: operand tiles of 64 columns x 128 rows (K-major) or
+// 64 columns x 64 rows (MN-major), whichever its products take, and epilogue chunks of 32 x 32.
+// Columns and rows past the matrix read as zero and are not written.
 struct Stack {
-  __half* data;
-  int rows, cols, ld;
-  long long batch;
-  CUtensorMap k_major, mn_major;
-  bool make(__half* ptr, int r, int c, int count) {
-    data = ptr;
-    rows = r, cols = c, ld = (c + 7) / 8 * 8;
-    batch = static_cast<long long>(rows) * ld;
-    return encode(&k_major, count, 128) && encode(&mn_major, count, 64);
+  CUtensorMap k_major, mn_major, chunk;
+  bool make(void* ptr, int rows, int cols, int count, bool k, bool mn) {
+    return (!k || encode(&k_major, ptr, rows, cols, count, 64, 128)) &&
+           (!mn || encode(&mn_major, ptr, rows, cols, count, 64, 64)) && encode(&chunk, ptr, rows, cols, count, 32, 32);
   }
-  bool encode(CUtensorMap* map, int count, cuuint32_t box_rows) {
+  static bool encode(CUtensorMap* map, void* ptr, int rows, int cols, int count, cuuint32_t box_cols, cuuint32_t box_rows) {
+    const cuuint64_t ld = static_cast<cuuint64_t>(cols + 7) / 8 * 16;
     cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(count)};
-    cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2, static_cast<cuuint64_t>(batch) * 2};
-    cuuint32_t box[3] = {64, box_rows, 1};
+    cuuint64_t strides[2] = {ld, ld * rows};
+    cuuint32_t box[3] = {box_cols, box_rows, 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    return g_encode_muon(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, data, dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return g_encode_muon(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, ptr, dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   }
+};
+// High and low parts.
+struct Pair {
+  Stack part[2];
 };
 
 int sms() {
@@ -752,7 +877,7 @@ int sms() {
 }
 
 template <int CG, bool SPLIT, bool A_MN, bool B_MN, int MODE>
-cudaError_t launch_product(const Stack* const (&a)[2], const Stack* const (&b)[2], GemmParams& p, int count,
+cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p, int count,
                            cudaStream_t stream) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
   constexpr int tile = BM * CG;
@@ -791,16 +916,22 @@ cudaError_t launch_product(const Stack* const (&a)[2], const Stack* const (&b)[2
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  auto map = [](const Stack* s, bool mn) -> const CUtensorMap& { return mn ? s->mn_major : s->k_major; };
-  return cudaLaunchKernelEx(&cfg, kern, map(a[0], A_MN), map(a[1], A_MN), map(b[0], B_MN), map(b[1], B_MN), p);
+  Maps maps;
+  for (int i = 0; i < 2; ++i) {
+    maps.a[i] = A_MN ? a.part[i].mn_major : a.part[i].k_major;
+    maps.b[i] = B_MN ? b.part[i].mn_major : b.part[i].k_major;
+    maps.c[i] = c.part[i].chunk;
+    maps.d[i] = d.part[i].chunk;
+  }
+  return cudaLaunchKernelEx(&cfg, kern, maps, p);
 }
 
 template <bool A_MN, bool B_MN, int MODE>
-cudaError_t product(int tile, bool split, const Stack* const (&a)[2], const Stack* const (&b)[2], GemmParams& p, int count,
-                    cudaStream_t s) {
-  if (split) return launch_product<1, true, A_MN, B_MN, MODE>(a, b, p, count, s);
-  return tile == 2 ? launch_product<2, false, A_MN, B_MN, MODE>(a, b, p, count, s)
-                   : launch_product<1, false, A_MN, B_MN, MODE>(a, b, p, count, s);
+cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p,
+                    int count, cudaStream_t s) {
+  if (split) return launch_product<1, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  return tile == 2 ? launch_product<2, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)
+                   : launch_product<1, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
 }
 
 struct Layout {  // byte offsets in the workspace (each 256-byte aligned)
@@ -868,14 +999,13 @@ extern "C" int md_muon(const MdMuonParams* prm, cudaStream_t stream) {
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
   const int small = p.rows < p.cols ? p.rows : p.cols;
   const bool tall = p.rows > p.cols, split = p.split != 0;
-  Stack x[2][2], a[2], f[2];
+  Pair x[2], a{}, f{};
   bool ok = true;
   for (int i = 0; i < 2; ++i)
-    for (int w = 0; w < 2; ++w)
-      ok = ok && x[i][w].make(reinterpret_cast<__half*>(ws + l.x[i][w]), p.rows, p.cols, p.count);
+    for (int w = 0; w < 2; ++w) ok = ok && x[i].part[w].make(ws + l.x[i][w], p.rows, p.cols, p.count, true, true);
   for (int w = 0; w <= static_cast<int>(split); ++w)
-    ok = ok && a[w].make(reinterpret_cast<__half*>(ws + l.a[w]), small, small, p.count) &&
-         f[w].make(reinterpret_cast<__half*>(ws + l.f[w]), small, small, p.count);
+    ok = ok && a.part[w].make(ws + l.a[w], small, small, p.count, true, false) &&
+         f.part[w].make(ws + l.f[w], small, small, p.count, true, false);
   if (!ok) return -8;
 
   cudaError_t e = p.step           ? prepare<float, true>(p, l, static_cast<int>(chunks), stream)
@@ -897,42 +1027,29 @@ extern "C" int md_muon(const MdMuonParams* prm, cudaStream_t stream) {
   g.decay = p.decay, g.rate = p.rate, g.lr = p.lr, g.skip = p.skip;
   for (int i = 0; i < p.count; ++i) g.out[i] = p.out[i], g.shadow[i] = p.step ? p.shadow[i] : nullptr;
   const float per = 1.f / kScale;
-  const Stack* as[2] = {&a[0], split ? &a[1] : &a[0]};
-  const Stack* fs[2] = {&f[0], split ? &f[1] : &f[0]};
-  auto put = [](const Stack& hi, const Stack* lo, __half* (&d)[2], long long& ld, long long& batch) {
-    d[0] = hi.data, d[1] = lo != nullptr ? lo->data : nullptr, ld = hi.ld, batch = hi.batch;
-  };
-  auto from = [](const Stack& hi, const Stack* lo, const __half* (&c)[2], long long& ld, long long& batch) {
-    c[0] = hi.data, c[1] = lo != nullptr ? lo->data : nullptr, ld = hi.ld, batch = hi.batch;
-  };
   for (int it = 0; it < p.iterations && e == cudaSuccess; ++it) {
     const bool last = it + 1 == p.iterations;
-    const Stack* xs[2] = {&x[it & 1][0], &x[it & 1][1]};
+    const Pair &xs = x[it & 1], &xn = x[~it & 1];
     // A = X X^T (X^T X)
     g.M = g.N = small, g.K = tall ? p.rows : p.cols;
     g.alpha = per, g.beta = 0.f;
-    put(a[0], split ? &a[1] : nullptr, g.d, g.ldd, g.batch_d);
-    e = tall ? product<true, true, kGram>(tile_sym, split, xs, xs, g, p.count, stream)
-             : product<false, false, kGram>(tile_sym, split, xs, xs, g, p.count, stream);
+    e = tall ? product<true, true, kGram>(tile_sym, split, xs, xs, a, a, g, p.count, stream)
+             : product<false, false, kGram>(tile_sym, split, xs, xs, a, a, g, p.count, stream);
     if (e != cudaSuccess) break;
     // B = b A + c A A
     g.K = small;
     g.alpha = p.c * per, g.beta = p.b;
-    from(a[0], split ? &a[1] : nullptr, g.c, g.ldc, g.batch_c);
-    put(f[0], split ? &f[1] : nullptr, g.d, g.ldd, g.batch_d);
-    e = product<false, false, kPoly>(tile_sym, split, as, as, g, p.count, stream);
+    e = product<false, false, kPoly>(tile_sym, split, a, a, a, f, g, p.count, stream);
     if (e != cudaSuccess) break;
     // X <- a X + B X (X B)
     g.M = p.rows, g.N = p.cols;
     g.alpha = per, g.beta = p.a;
-    from(*xs[0], xs[1], g.c, g.ldc, g.batch_c);
-    put(x[~it & 1][0], &x[~it & 1][1], g.d, g.ldd, g.batch_d);
     if (last)
-      e = tall ? product<false, false, kLast>(tile_all, split, xs, fs, g, p.count, stream)
-               : product<false, true, kLast>(tile_all, split, fs, xs, g, p.count, stream);
+      e = tall ? product<false, false, kLast>(tile_all, split, xs, f, xs, xn, g, p.count, stream)
+               : product<false, true, kLast>(tile_all, split, f, xs, xs, xn, g, p.count, stream);
     else
-      e = tall ? product<false, false, kNext>(tile_all, split, xs, fs, g, p.count, stream)
-               : product<false, true, kNext>(tile_all, split, fs, xs, g, p.count, stream);
+      e = tall ? product<false, false, kNext>(tile_all, split, xs, f, xs, xn, g, p.count, stream)
+               : product<false, true, kNext>(tile_all, split, f, xs, xs, xn, g, p.count, stream);
   }
   return static_cast<int>(e);
 }

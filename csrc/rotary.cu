@@ -14,11 +14,15 @@
 // into another tensor, at any batch / token / head stride, so q and k are
 // turned where the QKV projection left them.
 //
-// DRAM-bound: 2 bytes in and out per channel against three flops.  A thread
-// owns one vector (interleaved) or one pair of vectors R/2 apart (half) of a
-// token and walks up to kHeads heads with it, so a table entry is loaded once
-// for all of them and the loads of kHeads heads are in flight together.
+// DRAM-bound: 2 bytes in and out per channel against three flops, so what counts is
+// few instructions per byte and enough loads in flight.  A thread owns one unit of
+// a token (a vector, in the half layout the two vectors that turn together) for
+// four heads: cos and sin are loaded once for all four, the index arithmetic
+// (multiplications instead of divisions) is paid once, and the channels that pass
+// through are copied by the same threads in vectors of their own width.
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "md_sm100.cuh"
 
@@ -52,60 +56,125 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
 
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { using type = uint4; };
+template <> struct RawOf<8> { using type = uint2; };
+template <> struct RawOf<4> { using type = uint32_t; };
+template <> struct RawOf<2> { using type = uint16_t; };
+
+// VEC channels as loaded, and as fp32 (pairs are converted together).
 template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Vec {
-  T v[VEC];
+struct Vec {
+  using Raw = typename RawOf<sizeof(T) * VEC>::type;
+  static __device__ __forceinline__ void get(const Raw& raw, float (&f)[VEC]) {
+    const T* t = reinterpret_cast<const T*>(&raw);
+    if constexpr (sizeof(T) == 2 && VEC >= 2) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+#pragma unroll
+      for (int q = 0; q < VEC / 2; ++q) {
+        float2 v;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) v = unpack_bf16x2(w[q]);
+        else v = __half22float2(*reinterpret_cast<const __half2*>(w + q));
+        f[2 * q] = v.x, f[2 * q + 1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = to_f(t[j]);
+    }
+  }
+  static __device__ __forceinline__ Raw put(const float (&f)[VEC]) {
+    Raw raw;
+    if constexpr (sizeof(T) == 2 && VEC >= 2) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
+#pragma unroll
+      for (int q = 0; q < VEC / 2; ++q) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          w[q] = pack_bf16x2(f[2 * q], f[2 * q + 1]);
+        } else {
+          const __half2 h = __floats2half2_rn(f[2 * q], f[2 * q + 1]);
+          w[q] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+    } else {
+      T* t = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) t[j] = from_f<T>(f[j]);
+    }
+    return raw;
+  }
 };
 
-// One thread: unit `u` of a token, heads h0, h0 + 1, .. h0 + HEADS - 1 (q's heads first, then k's).
-// PAIRED: the unit is two vectors of VEC channels that turn together (the half layout; the
+// n / d and n mod d for n < 2^31 by one multiplication (d from the host; Granlund & Montgomery 1994).
+struct Divide {
+  unsigned d, mul, shift;
+  static Divide by(unsigned d) {
+    Divide v{d, 0, 0};
+    while ((1ull << v.shift) < d) ++v.shift;
+    v.mul = static_cast<unsigned>(((1ull << 32) * ((1ull << v.shift) - d)) / d + 1);
+    return v;
+  }
+  __device__ __forceinline__ unsigned operator()(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
+constexpr int kHeads = 4;  // heads per thread
+
+struct Shape {
+  unsigned total[2];   // threads with work, for q and for k
+  Divide units;        // units of a head
+  Divide groups[2];    // groups of kHeads heads, or single heads when there are few threads
+  Divide seq;
+  int per;             // heads of a group (kHeads or 1)
+  int pass_bytes;      // width of the pass-through vectors (16, 8, 4 or 2)
+  int pass;            // pass-through vectors of a head (0: in place)
+};
+
+template <typename W>
+__device__ __forceinline__ void copy_pass(const char* x, char* y, long long xs, long long ys, int n, int u, int units, int pass) {
+  for (int v = u; v < pass; v += units) {
+    W w[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+      if (i < n) w[i] = *reinterpret_cast<const W*>(x + i * xs + v * sizeof(W));
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+      if (i < n) *reinterpret_cast<W*>(y + i * ys + v * sizeof(W)) = w[i];
+  }
+}
+
+// PAIRED: a unit is two vectors of VEC channels that turn together (the half layout; the
 // interleaved layout with VEC = 1); otherwise one vector of VEC / 2 interleaved pairs.
-template <typename T, int VEC, bool HALF, int HEADS>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ MdRotaryParams p, int units, int rot_units,
-                                                     int head_groups, long long total) {
+template <typename T, int VEC, bool HALF>
+__global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ MdRotaryParams p,
+                                                     const __grid_constant__ Shape sh) {
   constexpr bool PAIRED = HALF || VEC == 1;
   constexpr int NCS = PAIRED ? VEC : VEC / 2;  // (cos, sin) entries a unit needs
   using V = Vec<T, VEC>;
+  using Raw = typename V::Raw;
   pdl_trigger();
   pdl_wait();
-  const long long id = blockIdx.x * 256ll + threadIdx.x;
-  if (id >= total) return;
-  const long long tg = id / units;
-  const int u = static_cast<int>(id - tg * units);
-  const long long token = tg / head_groups;
-  const int h0 = static_cast<int>(tg - token * head_groups) * HEADS;
-  const int b = static_cast<int>(token / p.seq), s = static_cast<int>(token - static_cast<long long>(b) * p.seq);
-  const int all = p.heads[0] + p.heads[1];
-  const bool turns = u < rot_units;
-
-  int c0, c1;  // first channel of the unit's vectors
-  if (!turns) c0 = c1 = p.rotary + (u - rot_units) * VEC;
-  else if (HALF) c0 = u * VEC, c1 = p.rotary / 2 + u * VEC;
-  else if (VEC == 1) c0 = 2 * u, c1 = 2 * u + 1;
-  else c0 = c1 = u * VEC;
-
-  V x0[HEADS], x1[HEADS];
-  const T* src[HEADS];
-  T* dst[HEADS];
+  const int w = blockIdx.y;  // q or k
+  const unsigned id = blockIdx.x * 256u + threadIdx.x;
+  if (id >= sh.total[w]) return;
+  const unsigned rest = sh.units(id);
+  const int u = static_cast<int>(id - rest * sh.units.d);
+  const unsigned token = sh.groups[w](rest);
+  const int h0 = static_cast<int>(rest - token * sh.groups[w].d) * sh.per;
+  const unsigned b = sh.seq(token);
+  const int s = static_cast<int>(token - b * sh.seq.d);
+  const int n = min(sh.per, p.heads[w] - h0);
+  const long long xs = p.xs[w][2], ys = p.ys[w][2];
+  const T* x = static_cast<const T*>(p.x[w]) + b * p.xs[w][0] + s * p.xs[w][1] + h0 * xs;
+  T* y = static_cast<T*>(p.y[w]) + b * p.ys[w][0] + s * p.ys[w][1] + h0 * ys;
+  // First channels of the unit's vectors.
+  const int c0 = HALF ? u * VEC : PAIRED ? 2 * u : u * VEC;
+  const int c1 = HALF ? p.rotary / 2 + u * VEC : PAIRED ? 2 * u + 1 : 0;
+  Raw r0[kHeads], r1[kHeads];
 #pragma unroll
-  for (int i = 0; i < HEADS; ++i) {
-    const int hh = h0 + i;
-    const int w = hh >= p.heads[0] ? 1 : 0;
-    const int h = hh - (w ? p.heads[0] : 0);
-    src[i] = static_cast<const T*>(w ? p.x[1] : p.x[0]) + b * (w ? p.xs[1][0] : p.xs[0][0]) +
-             s * (w ? p.xs[1][1] : p.xs[0][1]) + h * (w ? p.xs[1][2] : p.xs[0][2]);
-    dst[i] = static_cast<T*>(w ? p.y[1] : p.y[0]) + b * (w ? p.ys[1][0] : p.ys[0][0]) +
-             s * (w ? p.ys[1][1] : p.ys[0][1]) + h * (w ? p.ys[1][2] : p.ys[0][2]);
-    if (hh < all) {
-      x0[i] = *reinterpret_cast<const V*>(src[i] + c0);
-      if (PAIRED && turns) x1[i] = *reinterpret_cast<const V*>(src[i] + c1);
+  for (int i = 0; i < kHeads; ++i) {
+    if (i < n) {
+      r0[i] = *reinterpret_cast<const Raw*>(x + i * xs + c0);
+      if (PAIRED) r1[i] = *reinterpret_cast<const Raw*>(x + i * xs + c1);
     }
-  }
-  if (!turns) {
-#pragma unroll
-    for (int i = 0; i < HEADS; ++i)
-      if (h0 + i < all) *reinterpret_cast<V*>(dst[i] + c0) = x0[i];
-    return;
   }
 
   long long pos = s;
@@ -139,53 +208,68 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ MdR
     for (int q = 0; q < NCS; ++q) cs[2 * q + 1] = -cs[2 * q + 1];
   }
 #pragma unroll
-  for (int i = 0; i < HEADS; ++i) {
-    if (h0 + i >= all) break;
+  for (int i = 0; i < kHeads; ++i) {
+    if (i >= n) break;
+    T* dst = y + i * ys;
+    float a[VEC], c[VEC], o[VEC];
+    V::get(r0[i], a);
     if (PAIRED) {
+      V::get(r1[i], c);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float a = to_f(x0[i].v[j]), c = to_f(x1[i].v[j]);
-        x0[i].v[j] = from_f<T>(a * cs[2 * j] - c * cs[2 * j + 1]);
-        x1[i].v[j] = from_f<T>(c * cs[2 * j] + a * cs[2 * j + 1]);
-      }
-      *reinterpret_cast<V*>(dst[i] + c0) = x0[i];
-      *reinterpret_cast<V*>(dst[i] + c1) = x1[i];
+      for (int j = 0; j < VEC; ++j) o[j] = a[j] * cs[2 * j] - c[j] * cs[2 * j + 1];
+      *reinterpret_cast<Raw*>(dst + c0) = V::put(o);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) o[j] = c[j] * cs[2 * j] + a[j] * cs[2 * j + 1];
+      *reinterpret_cast<Raw*>(dst + c1) = V::put(o);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC / 2; ++j) {
-        const float a = to_f(x0[i].v[2 * j]), c = to_f(x0[i].v[2 * j + 1]);
-        x0[i].v[2 * j] = from_f<T>(a * cs[2 * j] - c * cs[2 * j + 1]);
-        x0[i].v[2 * j + 1] = from_f<T>(c * cs[2 * j] + a * cs[2 * j + 1]);
+        o[2 * j] = a[2 * j] * cs[2 * j] - a[2 * j + 1] * cs[2 * j + 1];
+        o[2 * j + 1] = a[2 * j + 1] * cs[2 * j] + a[2 * j] * cs[2 * j + 1];
       }
-      *reinterpret_cast<V*>(dst[i] + c0) = x0[i];
+      *reinterpret_cast<Raw*>(dst + c0) = V::put(o);
     }
+  }
+  if (sh.pass > 0) {
+    const char* px = reinterpret_cast<const char*>(x + p.rotary);
+    char* py = reinterpret_cast<char*>(y + p.rotary);
+    const long long xb = xs * static_cast<long long>(sizeof(T)), yb = ys * static_cast<long long>(sizeof(T));
+    const int units = static_cast<int>(sh.units.d);
+    if (sh.pass_bytes == 16) copy_pass<uint4>(px, py, xb, yb, n, u, units, sh.pass);
+    else if (sh.pass_bytes == 8) copy_pass<uint2>(px, py, xb, yb, n, u, units, sh.pass);
+    else if (sh.pass_bytes == 4) copy_pass<uint32_t>(px, py, xb, yb, n, u, units, sh.pass);
+    else copy_pass<uint16_t>(px, py, xb, yb, n, u, units, sh.pass);
   }
 }
 
-constexpr int kHeads = 4;
-
 template <typename T, int VEC, bool HALF>
-cudaError_t launch(const MdRotaryParams& p, bool in_place, cudaStream_t stream) {
+cudaError_t launch(const MdRotaryParams& p, bool in_place, int pass_bytes, cudaStream_t stream) {
   constexpr bool PAIRED = HALF || VEC == 1;
-  const int rot_units = PAIRED ? p.rotary / 2 / VEC : p.rotary / VEC;
-  const int units = rot_units + (in_place ? 0 : (p.dim - p.rotary) / VEC);
+  const int units = PAIRED ? p.rotary / 2 / VEC : p.rotary / VEC;
+  Shape sh;
+  sh.units = Divide::by(units);
+  sh.seq = Divide::by(p.seq);
+  sh.pass_bytes = pass_bytes;
+  sh.pass = in_place ? 0 : (p.dim - p.rotary) * static_cast<int>(sizeof(T)) / pass_bytes;
   const long long tokens = static_cast<long long>(p.batch) * p.seq;
-  const int all = p.heads[0] + p.heads[1];
   // One head per thread while that leaves SMs without work, four once the grid is larger.
-  const bool few = tokens * units * all < 148ll * 2048;
-  const int per = few ? 1 : kHeads;
-  const int groups = (all + per - 1) / per;
-  const long long total = tokens * groups * units;
-  const long long blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  const dim3 grid(static_cast<unsigned>(blocks));
-  return few ? launch_pdl(rotary_kernel<T, VEC, HALF, 1>, grid, dim3(256), 0, stream, p, units, rot_units, groups, total)
-             : launch_pdl(rotary_kernel<T, VEC, HALF, kHeads>, grid, dim3(256), 0, stream, p, units, rot_units, groups, total);
+  sh.per = tokens * units * (p.heads[0] + p.heads[1]) < 148ll * 2048 ? 1 : kHeads;
+  long long most = 0;
+  for (int w = 0; w < 2; ++w) {
+    const int groups = (p.heads[w] + sh.per - 1) / sh.per;
+    const long long total = tokens * groups * units;
+    if (total > 0x7fffff00ll) return cudaErrorInvalidConfiguration;
+    sh.groups[w] = Divide::by(groups > 0 ? groups : 1);
+    sh.total[w] = static_cast<unsigned>(total);
+    if (total > most) most = total;
+  }
+  const dim3 grid(static_cast<unsigned>((most + 255) / 256), p.heads[1] > 0 ? 2 : 1);
+  return launch_pdl(rotary_kernel<T, VEC, HALF>, grid, dim3(256), 0, stream, p, sh);
 }
 
 template <typename T, int VEC>
-cudaError_t pick_layout(const MdRotaryParams& p, bool in_place, cudaStream_t s) {
-  return p.interleaved ? launch<T, VEC, false>(p, in_place, s) : launch<T, VEC, true>(p, in_place, s);
+cudaError_t pick_layout(const MdRotaryParams& p, bool in_place, int pass_bytes, cudaStream_t s) {
+  return p.interleaved ? launch<T, VEC, false>(p, in_place, pass_bytes, s) : launch<T, VEC, true>(p, in_place, pass_bytes, s);
 }
 
 }  // namespace rotary
@@ -202,10 +286,9 @@ extern "C" int md_rotary(const MdRotaryParams* prm, cudaStream_t stream) {
   if (p.dtype < 0 || p.dtype > 2) return -5;
   if (p.batch == 0 || p.seq == 0 || p.heads[0] + p.heads[1] == 0) return 0;
   const int es = p.dtype == 2 ? 4 : 2;
-  // The widest vector that divides every offset a vector can start at: the tensors' addresses
-  // and strides, the head, its rotary part and, for the half layout, half of that.
-  unsigned long long bits = static_cast<unsigned long long>(p.dim) * es | static_cast<unsigned long long>(p.rotary) * es;
-  if (!p.interleaved) bits |= static_cast<unsigned long long>(p.rotary / 2) * es;
+  // The widest vectors that divide every offset one can start at: the tensors' addresses and strides,
+  // and the rotary part (half of it in the half layout) or, passing through, its end and the head's.
+  unsigned long long bits = 0;
   bool in_place = true;
   for (int w = 0; w < 2; ++w) {
     if (p.heads[w] == 0) continue;
@@ -217,23 +300,29 @@ extern "C" int md_rotary(const MdRotaryParams* prm, cudaStream_t stream) {
       if (p.xs[w][i] != p.ys[w][i]) in_place = false;
     }
   }
-  int vec = 1;
-  while (vec * es < 16 && bits % (2ull * vec * es) == 0) vec *= 2;
+  auto widest = [](unsigned long long offsets, int from) {
+    int w = from;
+    while (w < 16 && offsets % (2ull * w) == 0) w *= 2;
+    return w;
+  };
+  const unsigned long long turned = static_cast<unsigned long long>(p.interleaved ? p.rotary : p.rotary / 2) * es;
+  const int vec = widest(bits | turned, es) / es;
+  const int pass = widest(bits | static_cast<unsigned long long>(p.rotary) * es | static_cast<unsigned long long>(p.dim) * es, es);
   cudaError_t e;
   if (p.dtype == 0) {
-    e = vec == 8   ? pick_layout<__nv_bfloat16, 8>(p, in_place, stream)
-        : vec == 4 ? pick_layout<__nv_bfloat16, 4>(p, in_place, stream)
-        : vec == 2 ? pick_layout<__nv_bfloat16, 2>(p, in_place, stream)
-                   : pick_layout<__nv_bfloat16, 1>(p, in_place, stream);
+    e = vec == 8   ? pick_layout<__nv_bfloat16, 8>(p, in_place, pass, stream)
+        : vec == 4 ? pick_layout<__nv_bfloat16, 4>(p, in_place, pass, stream)
+        : vec == 2 ? pick_layout<__nv_bfloat16, 2>(p, in_place, pass, stream)
+                   : pick_layout<__nv_bfloat16, 1>(p, in_place, pass, stream);
   } else if (p.dtype == 1) {
-    e = vec == 8   ? pick_layout<__half, 8>(p, in_place, stream)
-        : vec == 4 ? pick_layout<__half, 4>(p, in_place, stream)
-        : vec == 2 ? pick_layout<__half, 2>(p, in_place, stream)
-                   : pick_layout<__half, 1>(p, in_place, stream);
+    e = vec == 8   ? pick_layout<__half, 8>(p, in_place, pass, stream)
+        : vec == 4 ? pick_layout<__half, 4>(p, in_place, pass, stream)
+        : vec == 2 ? pick_layout<__half, 2>(p, in_place, pass, stream)
+                   : pick_layout<__half, 1>(p, in_place, pass, stream);
   } else {
-    e = vec == 4   ? pick_layout<float, 4>(p, in_place, stream)
-        : vec == 2 ? pick_layout<float, 2>(p, in_place, stream)
-                   : pick_layout<float, 1>(p, in_place, stream);
+    e = vec == 4   ? pick_layout<float, 4>(p, in_place, pass, stream)
+        : vec == 2 ? pick_layout<float, 2>(p, in_place, pass, stream)
+                   : pick_layout<float, 1>(p, in_place, pass, stream);
   }
   return static_cast<int>(e);
 }

@@ -208,8 +208,9 @@ def check_status(device=None, reset: bool = True) -> None:
 
 
 def stream_ptr(stream: torch.cuda.Stream | None = None) -> int:
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return int(s.cuda_stream)
+    if stream is None:  # (the raw handle, without building a Stream object: this runs before every launch)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return int(stream.cuda_stream)
 
 
 _HERE = contextlib.nullcontext()

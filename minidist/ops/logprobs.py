@@ -15,7 +15,7 @@ the same arithmetic runs with torch operations.
 
 from __future__ import annotations
 
-import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -38,44 +38,25 @@ class TokenLogprobs(NamedTuple):
     top_tokens: torch.Tensor | None  # int64 [..., top]
 
 
-class _Params(ctypes.Structure):
-    """Mirror of ``struct MdLogprobsParams`` in csrc/logprobs.cu."""
-
-    _fields_ = [
-        ("logits", ctypes.c_void_p),
-        ("ld", ctypes.c_longlong),
-        ("dtype", ctypes.c_int),
-        ("rows", ctypes.c_int),
-        ("vocab", ctypes.c_int),
-        ("tokens", ctypes.c_void_p),
-        ("ignore", ctypes.c_longlong),
-        ("inv_t", ctypes.c_float),
-        ("top", ctypes.c_int),
-        ("want_entropy", ctypes.c_int),
-        ("logprob", ctypes.c_void_p),
-        ("entropy", ctypes.c_void_p),
-        ("top_logprob", ctypes.c_void_p),
-        ("top_token", ctypes.c_void_p),
-        ("row_max", ctypes.c_void_p),
-        ("row_log", ctypes.c_void_p),
-        ("g_logprob", ctypes.c_void_p),
-        ("g_entropy", ctypes.c_void_p),
-        ("g_top", ctypes.c_void_p),
-        ("dlogits", ctypes.c_void_p),
-        ("ldd", ctypes.c_longlong),
-        ("status", ctypes.c_void_p),
-    ]
+# struct MdLogprobsParams in csrc/logprobs.cu, field for field (native alignment): logits, ld, dtype,
+# rows, vocab, tokens, ignore, inv_t, top, want_entropy, logprob, entropy, top_logprob, top_token,
+# row_max, row_log, g_logprob, g_entropy, g_top, dlogits, ldd, status.
+_PARAMS = struct.Struct("@Pq3iPqf2iPPPPPPPPPPqP")
 
 
-def _params(logits, tokens, temperature, top, entropy, ignore_index) -> _Params:
-    p = _Params()
-    rows, vocab = logits.shape
-    p.logits, p.ld, p.dtype = logits.data_ptr(), logits.stride(0), _DTYPE_CODE[logits.dtype]
-    p.rows, p.vocab = rows, vocab
-    p.tokens, p.ignore = tokens.data_ptr(), ignore_index
-    p.inv_t, p.top, p.want_entropy = 1.0 / temperature, top, entropy
-    p.status = nat.status_ptr(logits.device)
-    return p
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _call(entry, logits, tokens, temperature, top, ignore_index, logprob, h, top_lp, top_id, stats,
+          g=None, gh=None, gt=None, out=None):
+    row_max = _ptr(stats)
+    params = _PARAMS.pack(logits.data_ptr(), logits.stride(0), _DTYPE_CODE[logits.dtype], *logits.shape,
+                          tokens.data_ptr(), ignore_index, 1.0 / temperature, top, h is not None, _ptr(logprob),
+                          _ptr(h), _ptr(top_lp), _ptr(top_id), row_max, row_max and row_max + 4 * logits.shape[0], _ptr(g), _ptr(gh),
+                          _ptr(gt), _ptr(out), 0 if out is None else out.stride(0), nat.status_ptr(logits.device))
+    with nat.on_device(logits):
+        nat.check(getattr(nat.lib(), entry)(params, nat.stream_ptr()), entry)
 
 
 def _forward(logits, tokens, temperature, top, entropy, ignore_index, for_backward):
@@ -83,69 +64,56 @@ def _forward(logits, tokens, temperature, top, entropy, ignore_index, for_backwa
     new = logits.new_empty
     logprob = new(rows, dtype=torch.float32)
     h = new(rows, dtype=torch.float32) if entropy else None
-    row_max, row_log = new(2, rows, dtype=torch.float32) if for_backward else (None, None)
+    stats = new(2, rows, dtype=torch.float32) if for_backward else None  # per row: maximum, log of the sum
     top_lp = top_id = None
     if top:
         top_lp = torch.empty(rows, top, dtype=torch.float32, device=logits.device)
         top_id = torch.empty(rows, top, dtype=torch.int64, device=logits.device)
     if rows:
-        p = _params(logits, tokens, temperature, top, entropy, ignore_index)
-        p.logprob = logprob.data_ptr()
-        if entropy:
-            p.entropy = h.data_ptr()
-        if top:
-            p.top_logprob, p.top_token = top_lp.data_ptr(), top_id.data_ptr()
-        if for_backward:
-            p.row_max, p.row_log = row_max.data_ptr(), row_log.data_ptr()
-        with nat.on_device(logits):
-            nat.check(nat.lib().md_logprobs(ctypes.addressof(p), nat.stream_ptr()), "md_logprobs")
-    return logprob, h, top_lp, top_id, row_max, row_log
+        _call("md_logprobs", logits, tokens, temperature, top, ignore_index, logprob, h, top_lp, top_id, stats)
+    return logprob, h, top_lp, top_id, stats
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature, top, entropy, ignore_index):
         ctx.set_materialize_grads(False)
-        logprob, h, top_lp, top_id, row_max, row_log = _forward(logits, tokens, temperature, top, entropy,
-                                                                ignore_index, True)
-        ctx.save_for_backward(logits, tokens, h, top_id, row_max, row_log)
-        ctx.how = (temperature, top, ignore_index)
+        logprob, h, top_lp, top_id, stats = _forward(logits, tokens, temperature, top, entropy, ignore_index, True)
+        ctx.save_for_backward(logits, tokens, h, top_id)
+        ctx.how = (temperature, top, ignore_index, stats)
         if top_id is not None:
             ctx.mark_non_differentiable(top_id)
         return logprob, h, top_lp, top_id
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g, gh, gt, _):
-        logits, tokens, h, top_id, row_max, row_log = ctx.saved_tensors
-        temperature, top, ignore_index = ctx.how
-        rows, vocab = logits.shape
-        # The kernel's vectors start equally far from a 16-byte boundary in logits and gradient: rows
-        # keep the logits' padding modulo 16 bytes (the LM head's padded rows stay aligned) and the
-        # first one its offset.
-        per = 16 // logits.element_size()
-        ld = vocab + (logits.stride(0) - vocab) % per
-        shift = logits.data_ptr() % 16 // logits.element_size()
-        out = logits.new_empty(rows * ld + shift)[shift:].view(rows, ld)[:, :vocab]
-        if rows and (g is not None or gh is not None or gt is not None):
-            p = _params(logits, tokens, temperature, top, h is not None, ignore_index)
-            p.row_max, p.row_log = row_max.data_ptr(), row_log.data_ptr()
-            if g is not None:
-                g = g.float().contiguous()
-                p.g_logprob = g.data_ptr()
-            if gh is not None:
-                gh = gh.float().contiguous()
-                p.g_entropy, p.entropy = gh.data_ptr(), h.data_ptr()
-            if gt is not None:
-                gt = gt.float().contiguous()
-                p.g_top, p.top_token = gt.data_ptr(), top_id.data_ptr()
-            p.dlogits, p.ldd = out.data_ptr(), ld
-            with nat.on_device(logits):
-                nat.check(nat.lib().md_logprobs_backward(ctypes.addressof(p), nat.stream_ptr()),
-                          "md_logprobs_backward")
-        else:
-            out.zero_()
-        return out, None, None, None, None, None
+    def backward(ctx, *grads):
+        # (once_differentiable's wrapper only where a second derivative could be asked for)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, *grads)
+
+
+def _backward(ctx, g, gh, gt, _):
+    logits, tokens, h, top_id = ctx.saved_tensors
+    temperature, top, ignore_index, stats = ctx.how
+    rows, vocab = logits.shape
+    # The kernel's vectors start equally far from a 16-byte boundary in logits and gradient: rows keep
+    # the logits' padding modulo 16 bytes (the LM head's padded rows stay aligned) and the first one
+    # its offset.
+    size = logits.element_size()
+    ld = vocab + (logits.stride(0) - vocab) % (16 // size)
+    shift = logits.data_ptr() % 16 // size
+    out = logits.new_empty(rows * ld + shift)[shift:].view(rows, ld) if shift else logits.new_empty(rows, ld)
+    if ld != vocab:
+        out = out[:, :vocab]
+    if rows and (g is not None or gh is not None or gt is not None):
+        g, gh, gt = (None if t is None else t.float().contiguous() for t in (g, gh, gt))
+        _call("md_logprobs_backward", logits, tokens, temperature, top, ignore_index, None, h, None, top_id, stats,
+              g, gh, gt, out)
+    else:
+        out.zero_()
+    return out, None, None, None, None, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class _Lookup(torch.autograd.Function):
@@ -220,12 +188,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
         raise ValueError(f"token_logprobs: temperature {temperature} is not positive and finite")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"token_logprobs: top={top} is not within [0, {min(MAX_TOP, vocab)}]")
-    flat = logits.reshape(-1, vocab)
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     if flat.stride(1) != 1 or (flat.shape[0] > 1 and flat.stride(0) < vocab):
         flat = flat.contiguous()
     elif flat.shape[0] <= 1 and flat.stride(0) < vocab:
         flat = flat.as_strided(flat.shape, (vocab, 1))
-    ids = tokens.reshape(-1).contiguous()
+    ids = tokens.contiguous() if tokens.dim() == 1 else tokens.reshape(-1).contiguous()
     need = logits.requires_grad and torch.is_grad_enabled()
     if not logits.is_cuda:
         out = _Lookup.apply(flat, ids, temperature, top, entropy, ignore_index)

@@ -13,8 +13,8 @@ differentiate (the gradient is the rotation back).
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -79,53 +79,30 @@ def rotary_table(rotary_dim: int, positions: int, *, base: float = 10000.0, scal
     return (torch.stack([angle.cos(), angle.sin()], dim=-1) * scale).float()
 
 
-class _Params(ctypes.Structure):
-    """Mirror of ``struct MdRotaryParams`` in csrc/rotary.cu."""
-
-    _fields_ = [
-        ("x", ctypes.c_void_p * 2),
-        ("y", ctypes.c_void_p * 2),
-        ("xs", (ctypes.c_longlong * 3) * 2),
-        ("ys", (ctypes.c_longlong * 3) * 2),
-        ("heads", ctypes.c_int * 2),
-        ("table", ctypes.c_void_p),
-        ("table_rows", ctypes.c_longlong),
-        ("positions", ctypes.c_void_p),
-        ("positions64", ctypes.c_int),
-        ("ps", ctypes.c_longlong * 2),
-        ("batch", ctypes.c_int),
-        ("seq", ctypes.c_int),
-        ("dim", ctypes.c_int),
-        ("rotary", ctypes.c_int),
-        ("interleaved", ctypes.c_int),
-        ("inverse", ctypes.c_int),
-        ("dtype", ctypes.c_int),
-        ("status", ctypes.c_void_p),
-    ]
+# struct MdRotaryParams in csrc/rotary.cu, field for field (native alignment): x[2], y[2], xs[2][3],
+# ys[2][3], heads[2], table, table_rows, positions, positions64, ps[2], batch, seq, dim, rotary,
+# interleaved, inverse, dtype, status.
+_PARAMS = struct.Struct("@2P2P6q6q2iPqPi2q7iP")
 
 
 def _launch(q, k, q_out, k_out, table, positions, interleaved: bool, inverse: bool) -> None:
     B, S, H, D = q.shape
-    p = _Params()
-    p.x[0], p.y[0] = q.data_ptr(), q_out.data_ptr()
-    p.xs[0][:] = q.stride()[:3]
-    p.ys[0][:] = q_out.stride()[:3]
-    p.heads[0] = H
-    if k is not None:
-        p.x[1], p.y[1] = k.data_ptr(), k_out.data_ptr()
-        p.xs[1][:] = k.stride()[:3]
-        p.ys[1][:] = k_out.stride()[:3]
-        p.heads[1] = k.shape[2]
-    p.table, p.table_rows = table.data_ptr(), table.shape[0]
-    if positions is not None:
-        p.positions, p.positions64 = positions.data_ptr(), positions.dtype == torch.int64
-        st = positions.stride()
-        p.ps[:] = (0, st[0]) if positions.dim() == 1 else st
-    p.batch, p.seq, p.dim, p.rotary = B, S, D, 2 * table.shape[1]
-    p.interleaved, p.inverse, p.dtype = interleaved, inverse, _DTYPE_CODE[q.dtype]
-    p.status = nat.status_ptr(q.device)
+    xs, ys = q.stride()[:3], q_out.stride()[:3]
+    if k is None:
+        kp, kop, Hk, kxs, kys = 0, 0, 0, (0, 0, 0), (0, 0, 0)
+    else:
+        kp, kop, Hk, kxs, kys = k.data_ptr(), k_out.data_ptr(), k.shape[2], k.stride()[:3], k_out.stride()[:3]
+    if positions is None:
+        pos, wide, ps = 0, 0, (0, 0)
+    else:
+        pos, wide, ps = positions.data_ptr(), positions.dtype == torch.int64, positions.stride()
+        if len(ps) == 1:
+            ps = (0, ps[0])
+    params = _PARAMS.pack(q.data_ptr(), kp, q_out.data_ptr(), kop, *xs, *kxs, *ys, *kys, H, Hk, table.data_ptr(),
+                          table.shape[0], pos, wide, *ps, B, S, D, 2 * table.shape[1], interleaved, inverse,
+                          _DTYPE_CODE[q.dtype], nat.status_ptr(q.device))
     with nat.on_device(q):
-        nat.check(nat.lib().md_rotary(ctypes.addressof(p), nat.stream_ptr()), "md_rotary")
+        nat.check(nat.lib().md_rotary(params, nat.stream_ptr()), "md_rotary")
 
 
 def _turn_cpu(x, table, positions, interleaved, inverse):
@@ -154,8 +131,8 @@ def _turn(q, k, table, positions, interleaved, inverse, inplace=False):
         q_out, k_out = q, k
     else:
         q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (q, k))
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     _launch(q, k, q_out, k_out, table, positions, interleaved, inverse)
     return [q_out, k_out]
 
@@ -172,12 +149,11 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dq, dk):
         table, positions = ctx.saved_tensors
         interleaved, inverse = ctx.how
-        if dq is None and dk is None:
-            return (None,) * 6
-        if dq is None:
-            (dk, _) = _Rotary.apply(dk, None, table, positions, interleaved, not inverse)
-        else:
-            dq, dk = _Rotary.apply(dq, dk, table, positions, interleaved, not inverse)
+        turn = _Rotary.apply if torch.is_grad_enabled() else _turn  # (differentiable again if asked for)
+        if dq is not None:
+            dq, dk = turn(dq, dk, table, positions, interleaved, not inverse)
+        elif dk is not None:
+            dk, _ = turn(dk, None, table, positions, interleaved, not inverse)
         return dq, dk, None, None, None, None
 
 

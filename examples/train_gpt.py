@@ -11,8 +11,13 @@ Flags match the reference trainer (examples/train_gpt.py:59-92):
 On B200 with ``--precision bf16`` every block runs on the hand-written sm_100a
 kernels and gradients are averaged by the peer-memory all-reduce; with
 ``--precision fp32`` (or on CPU) the portable path runs.  Added flags:
-``--optimizer {auto,fused,torch}`` and ``--timing {device,host}`` (device =
-CUDA-event step time, maximum over ranks, the default on GPU).
+``--optimizer {auto,fused,torch,muon}`` and ``--timing {device,host}`` (device =
+CUDA-event step time, maximum over ranks, the default on GPU);
+``--positions rotary`` for rotary instead of learned positions and
+``--score-every N`` for the log probabilities, entropy and ranks that the model
+gives a batch's targets:
+
+    torchrun --nproc-per-node 1 examples/train_gpt.py --precision bf16 --positions rotary --optimizer muon --score-every 5
 
 The data are synthetic uniform-random tokens, seeded by
 ``seed + step*10000 + dp_rank`` so tensor/pipeline peers see identical batches
@@ -51,6 +56,7 @@ from minidist import (  # noqa: E402
     resolve_precision,
     shutdown_distributed,
     summarize_collectives,
+    token_logprobs,
 )
 from minidist.fsdp import MixedPrecisionPolicy  # noqa: E402
 from minidist.models import GPT, Block, GPTConfig, LMHead, build_pipeline_layers  # noqa: E402
@@ -78,14 +84,20 @@ def parse_args(argv=None) -> argparse.Namespace:
     model.add_argument("--vocab", type=int, default=8192)
     model.add_argument("--seq-len", type=int, default=256)
     model.add_argument("--batch-size", type=int, default=16, help="per data-parallel replica")
+    model.add_argument("--positions", default="learned", choices=["learned", "rotary"])
+    model.add_argument("--rotary-fraction", type=float, default=1.0, help="share of each head's channels that turn")
     run = p.add_argument_group("run")
     run.add_argument("--steps", type=int, default=20)
     run.add_argument("--lr", type=float, default=3e-4)
     run.add_argument("--seed", type=int, default=1234)
     run.add_argument("--profile", metavar="PATH", default=None,
                      help="export a Chrome trace (one per rank) and print an overlap report")
-    run.add_argument("--optimizer", default="auto", choices=["auto", "fused", "torch"],
-                     help="AdamW implementation (fused = multi-tensor sm_100a kernel)")
+    run.add_argument("--optimizer", default="auto", choices=["auto", "fused", "torch", "muon"],
+                     help="AdamW implementation (fused = multi-tensor sm_100a kernel), or muon: orthogonalised "
+                          "updates for the blocks' matrices, fused AdamW for the rest")
+    run.add_argument("--score-every", type=int, default=0, metavar="N",
+                     help="every N steps print the mean log probability and entropy of the batch's targets and "
+                          "how often a target is among the 5 likeliest tokens (no pipeline, no tensor parallelism)")
     run.add_argument("--timing", default="auto", choices=["auto", "device", "host"])
     run.add_argument("--save", metavar="DIR", default=None, help="write a checkpoint here at the end")
     run.add_argument("--kernels", default="fused", choices=["fused", "nccl"],
@@ -163,6 +175,10 @@ def build(args, mesh: ParallelMesh, config: GPTConfig, device, precision):
 
 def make_optimizer(args, model, device):
     params = list(model.parameters())
+    if args.optimizer == "muon":
+        from minidist.optim import Muon, muon_groups
+
+        return Muon(muon_groups(model), lr=args.lr, capturable=args.cuda_graph)
     use_fused = args.optimizer == "fused" or args.cuda_graph or (
         args.optimizer == "auto" and device.type == "cuda" and all(p.dtype == torch.float32 for p in params))
     if use_fused:
@@ -200,7 +216,8 @@ def main(argv=None) -> None:
     torch.manual_seed(args.seed)
     mesh = ParallelMesh(tp_size=args.tp, pp_size=args.pp)
     config = GPTConfig(vocab_size=args.vocab, block_size=args.seq_len, n_layer=args.layers, n_head=args.heads,
-                       n_embd=args.embd, seed=args.seed)
+                       n_embd=args.embd, seed=args.seed, positions=args.positions,
+                       rotary_fraction=args.rotary_fraction)
     precision = resolve_precision(args.precision, device)
     device_timing = args.timing == "device" or (args.timing == "auto" and device.type == "cuda")
 
@@ -212,6 +229,10 @@ def main(argv=None) -> None:
                 + (f"pipeline: {args.schedule} x{args.microbatches}" if mesh.pp_size > 1 else ""))
     print_rank0("=" * 74)
 
+    if args.optimizer == "muon" and args.strategy == "fsdp" and mesh.dp_size > 1:
+        raise SystemExit("--optimizer muon needs whole matrices: FSDP keeps flat shards of them")
+    if args.score_every and (mesh.pp_size > 1 or mesh.tp_size > 1):
+        raise SystemExit("--score-every needs the whole model and vocabulary on every rank (pp = tp = 1)")
     model, core, loss_fn = build(args, mesh, config, device, precision)
     optimizer = make_optimizer(args, model, device)
     scaler = DistributedGradScaler(enabled=precision.needs_grad_scaler)
@@ -268,6 +289,15 @@ def main(argv=None) -> None:
         scaler.update()
         return value
 
+    def score(step: int) -> dict:
+        """How the model rates the batch's targets: token log probabilities, entropy, five best."""
+        ids, targets = make_batch(config, args.batch_size, mesh.dp_rank, step, args.seed, device)
+        with torch.no_grad(), precision.autocast():
+            logits = core(ids)
+        r = token_logprobs(logits, targets, top=min(5, config.vocab_size), entropy=True)
+        hit = (r.top_tokens == targets[..., None]).any(-1).float().mean()
+        return {"logprob": float(r.logprobs.mean()), "entropy": float(r.entropy.mean()), "top5": float(hit)}
+
     train_step(0)  # warm-up: communicator creation, allocator growth, kernel attributes
     if device.type == "cuda":
         torch.cuda.synchronize()
@@ -288,6 +318,11 @@ def main(argv=None) -> None:
                         f"{tokens_per_step * step / el:>9.0f} tok/s")
             metrics.write(step=step, loss=loss, ms_per_step=el / step * 1e3, tokens_per_s=tokens_per_step * step / el,
                           timing="host, rank 0")
+        if args.score_every and step % args.score_every == 0:
+            s = score(step)
+            print_rank0(f"  step {step:>4}/{args.steps}  targets: mean log p {s['logprob']:.4f}  entropy "
+                        f"{s['entropy']:.4f}  among the five likeliest {100 * s['top5']:.2f}%")
+            metrics.write(event="score", step=step, **s)
     if device.type == "cuda":
         torch.cuda.synchronize()
     total = time.perf_counter() - start

@@ -7,6 +7,7 @@ forward of a block (``M = batch*seq`` rows, bf16 activations)::
 
     h1, mu1, r1 = LayerNorm(x)                      md_ln_fwd
     qkv         = h1 Wqkv^T + bqkv                  tcgen05 GEMM, bias epilogue
+    (q, k turned in place by their positions        md_rotary, with rotary positions)
     y, lse      = causal attention(qkv)             md_attn_fwd
     x1          = x + y Wproj^T + bproj             GEMM, bias + residual epilogue
     h2, mu2, r2 = LayerNorm(x1)
@@ -46,6 +47,7 @@ from ..ops import _native as nat
 from ..ops import gemm as G
 from ..ops import grads as gradsink
 from ..ops import kernels as K
+from ..ops.rotary import rotate_packed_
 
 _SHADOW = "_md_bf16"
 _SHADOW_VER = "_md_bf16_ver"
@@ -247,13 +249,13 @@ class _EmbeddingFn(torch.autograd.Function):
         group = emb.group
         tp = _tp_world(group)
         x = None
-        if tp > 1:
+        if tp > 1 and wpe is not None:
             from ..parallel import collectives
 
             # Each row read from the rank that owns its vocabulary range (no reduction).
             x = collectives.embedding_tp(ids, wte, bf16_weight(wpe)[:S], group)
         if x is None:
-            add_pos = tp == 1 or emb.rank == 0  # positions summed once across the TP reduction
+            add_pos = wpe is not None and (tp == 1 or emb.rank == 0)  # positions summed once across the TP reduction
             x = K.embedding_fwd(ids, bf16_weight(wte), bf16_weight(wpe)[:S] if add_pos else None, S,
                                 vocab_start=emb.vocab_start if tp > 1 else 0)
             if tp > 1:
@@ -321,6 +323,9 @@ class _BlockFn(torch.autograd.Function):
 
         h1, mu1, r1 = K.layernorm_fwd(xin, ln1g, ln1b, blk.ln1.eps)
         qkv = G.linear_fwd(h1, w_qkv, qkv_b)
+        table = attn.rotary(xin.device)
+        if table is not None:
+            rotate_packed_(qkv, H, table, batch=B)
         y, lse = K.attention_fwd(qkv, B, S, H, D)
         if tp == 1:
             x1 = G.linear_fwd(y, w_proj, proj_b, resid=xin)
@@ -398,6 +403,9 @@ class _BlockFn(torch.autograd.Function):
         else:
             dy = G.linear_dgrad(dx1, w_proj)
         dqkv = K.attention_bwd(qkv, y, dy, lse, B, S, H, D, delta=delta)
+        table = attn.rotary(dqkv.device)
+        if table is not None:
+            rotate_packed_(dqkv, H, table, batch=B, inverse=True)
         # QKV (column-parallel)
         t_qw, t_qb = _targets(attn.qkv.weight, attn.qkv.bias)
         if t_qw is not None:

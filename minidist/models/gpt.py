@@ -2,7 +2,8 @@
 
 Architecture and parameter layout follow the reference (models/gpt.py:48-263)
 so checkpoints are interchangeable: pre-LayerNorm blocks (eps 1e-5), learned
-positions, GELU(tanh) MLP of width ``4*n_embd``, an *untied* LM head, and a QKV
+positions (or, with ``positions="rotary"``, queries and keys turned by their
+position and no ``wpe``), GELU(tanh) MLP of width ``4*n_embd``, an *untied* LM head, and a QKV
 projection whose output rows are interleaved per head as ``[n_head, 3,
 head_dim]`` so that any contiguous column-parallel slice holds whole heads with
 their own q, k and v (reference gpt.py:92-99).  Parameter names:
@@ -32,6 +33,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from .. import comm
+from ..ops.rotary import RotaryScaling, apply_rotary, rotary_table
 from ..tensor_parallel import (
     ColumnParallelLinear,
     RowParallelLinear,
@@ -52,6 +54,21 @@ class GPTConfig:
     dropout: float = 0.0
     bias: bool = True
     seed: int = 1234
+    positions: str = "learned"  # or "rotary"
+    rotary_fraction: float = 1.0  # share of each head's channels that turn
+    rotary_base: float = 10000.0
+    rotary_scaling: RotaryScaling | None = None
+
+    def __post_init__(self):
+        if self.positions not in ("learned", "rotary"):
+            raise ValueError(f"positions={self.positions!r}: expected 'learned' or 'rotary'")
+        if self.positions == "rotary" and (not 0.0 < self.rotary_fraction <= 1.0 or self.rotary_dim < 2):
+            raise ValueError(f"rotary_fraction={self.rotary_fraction} leaves no pair of {self.head_dim} channels to turn")
+
+    @property
+    def rotary_dim(self) -> int:
+        """Channels of a head that turn (an even number)."""
+        return int(self.head_dim * self.rotary_fraction) // 2 * 2
 
     @property
     def head_dim(self) -> int:
@@ -61,7 +78,8 @@ class GPTConfig:
         """Parameters of the untied model (embeddings + blocks + final LN + head)."""
         n, v = self.n_embd, self.vocab_size
         per_block = 12 * n * n + 4 * n + (9 * n if self.bias else 0)
-        return v * n + self.block_size * n + self.n_layer * per_block + n * v + 2 * n
+        positions = self.block_size * n if self.positions == "learned" else 0
+        return v * n + positions + self.n_layer * per_block + n * v + 2 * n
 
     def flops_per_token(self, seq_len: int | None = None) -> float:
         """Training FLOPs per token: 6 x matmul params + causal attention (fwd 2*S*n per layer x 3)."""
@@ -88,14 +106,30 @@ class CausalSelfAttention(nn.Module):
             raise ValueError(f"n_head={config.n_head} not divisible by tp_size={tp}")
         self.n_head_local = config.n_head // tp
         self.head_dim = config.head_dim
+        self.config = config
+        self._rotary: torch.Tensor | None = None
         self.qkv = ColumnParallelLinear(config.n_embd, 3 * config.n_embd, bias=config.bias, group=tp_group,
                                         seed=_seed_for(config, layer, 0), device=device, dtype=dtype)
         self.proj = RowParallelLinear(config.n_embd, config.n_embd, bias=config.bias, input_is_parallel=True,
                                       group=tp_group, seed=_seed_for(config, layer, 1), device=device, dtype=dtype)
 
+    def rotary(self, device) -> torch.Tensor | None:
+        """cos / sin of every position (None with learned positions); made on first use, not a parameter
+        or buffer, so checkpoints do not hold it."""
+        c = self.config
+        if c.positions != "rotary":
+            return None
+        if self._rotary is None or self._rotary.device != device:
+            self._rotary = rotary_table(c.rotary_dim, c.block_size, base=c.rotary_base, scaling=c.rotary_scaling,
+                                        device=device)
+        return self._rotary
+
     def forward(self, x):
         B, S, _ = x.shape
         q, k, v = self.qkv(x).view(B, S, self.n_head_local, 3, self.head_dim).unbind(dim=3)
+        table = self.rotary(x.device)
+        if table is not None:
+            q, k = apply_rotary(q, k, table)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
         return self.proj(y.transpose(1, 2).reshape(B, S, self.n_head_local * self.head_dim))
 
@@ -134,13 +168,16 @@ class Block(nn.Module):
 
 
 class Embedding(nn.Module):
-    """Token + learned position embedding (the first pipeline stage)."""
+    """Token (+ learned position) embedding (the first pipeline stage)."""
 
     def __init__(self, config: GPTConfig, tp_group=None, device=None, dtype=None):
         super().__init__()
         self.tp_group = tp_group
         self.wte = VocabParallelEmbedding(config.vocab_size, config.n_embd, group=tp_group,
                                           seed=_seed_for(config, -1, 0), device=device, dtype=dtype)
+        if config.positions == "rotary":
+            self.register_parameter("wpe", None)
+            return
         gen = torch.Generator(device="cpu").manual_seed(_seed_for(config, -1, 1))
         pos = torch.empty(config.block_size, config.n_embd).normal_(0.0, 0.02, generator=gen)
         self.wpe = nn.Parameter(pos.to(device=device, dtype=dtype))
@@ -150,7 +187,8 @@ class Embedding(nn.Module):
 
         if fused_gpt.should_fuse(input_ids):
             return fused_gpt.embedding_forward(self, input_ids)
-        return self.wte(input_ids) + self.wpe[: input_ids.size(1)]
+        x = self.wte(input_ids)
+        return x if self.wpe is None else x + self.wpe[: input_ids.size(1)]
 
 
 class LMHead(nn.Module):

@@ -12,6 +12,10 @@ memory ([lr, t]; the kernel computes the bias corrections), so a training step
 captured in a CUDA graph (:class:`minidist.graphs.GraphedStep`) advances the
 step on every replay; :meth:`FusedAdamW.sync_hyperparams` refreshes the device
 learning rate from ``param_groups`` between replays.
+
+:class:`Muon` is FusedAdamW with orthogonalised momentum updates
+(:mod:`minidist.ops.muon`) for the parameter groups that hold matrices;
+:func:`muon_groups` sorts a model's parameters into the two kinds of group.
 """
 
 from __future__ import annotations
@@ -23,8 +27,9 @@ import torch
 from .ddp import wait_handle
 from .ops import _native as nat
 from .ops import grads as gradsink
+from .ops import muon as muon_ops
 
-__all__ = ["FusedAdamW"]
+__all__ = ["FusedAdamW", "Muon", "muon_groups"]
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -97,6 +102,11 @@ class FusedAdamW(torch.optim.Optimizer):
         checked with torch ops)."""
         for gi, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
+            if group.get("orthogonal"):
+                self._wait_for(params)
+                for p in params:
+                    flag.add_((~torch.isfinite(p.grad)).any().to(flag.dtype).to(flag.device))
+                continue
             fused = [p for p in params if p.is_cuda and p.dtype == torch.float32 and p.grad.dtype == torch.float32]
             fused_ids = {id(p) for p in fused}
             for p in params:
@@ -132,6 +142,9 @@ class FusedAdamW(torch.optim.Optimizer):
         for gi, group in enumerate(self.param_groups):
             params = [p for p in group["params"] if p.grad is not None]
             if not params:
+                continue
+            if group.get("orthogonal"):
+                self._orthogonal_step(gi, group, params, inv_scale, skip)
                 continue
             self._init_states(params)
             states = [self._state(p) for p in params]
@@ -191,6 +204,15 @@ class FusedAdamW(torch.optim.Optimizer):
                 denom = st["exp_avg_sq"].sqrt().div_(bc2_sqrt).add_(eps)
                 p.addcdiv_(st["exp_avg"], denom, value=-lr / bc1)
         return loss
+
+    @staticmethod
+    def _wait_for(params) -> None:
+        """Order the current stream after the gradient reductions of ``params`` that are in flight."""
+        late = [p for p in params if getattr(p, "_md_grad_event", None) is not None]
+        for ev in {id(p._md_grad_event): p._md_grad_event for p in late}.values():
+            wait_handle(ev)
+        for p in late:
+            p._md_grad_event = None
 
     def _ensure_grad_buffers(self) -> None:
         """Give every CUDA fp32 parameter without one a persistent gradient buffer.
@@ -263,3 +285,99 @@ class FusedAdamW(torch.optim.Optimizer):
             cached = (key, table, chunk_t, len(chunks), table_h, chunk_h)
             self._tables[gi] = cached
         return cached[1], cached[2], cached[3]
+
+
+class Muon(FusedAdamW):
+    """Muon (Jordan et al. 2024) for matrices, AdamW for everything else, in one optimizer.
+
+    A group with ``orthogonal=True`` holds 2-D fp32 parameters; each takes
+    ``w = (1 - lr weight_decay) w - lr rms sqrt(max(rows, cols)) X`` where ``X`` is the
+    orthogonalised momentum (:func:`minidist.ops.muon.muon_update_`).  ``rms`` is the size of an
+    update's entries per unit of ``lr``; 0.2, about AdamW's, lets both kinds of group share a
+    learning rate.  Other groups are FusedAdamW's.  A group that does not say is orthogonal if all its
+    parameters are matrices::
+
+        opt = Muon(muon_groups(model), lr=3e-4)
+
+    State: ``momentum_buffer`` per matrix, AdamW's elsewhere.  Under tensor parallelism a shard is
+    orthogonalised as a matrix of its own; FSDP's flat shards are refused.  The loss scaler, deferred
+    DDP buckets and ``capturable=True`` work as with FusedAdamW.
+    """
+
+    def __init__(self, params, lr: float = 3e-4, *, momentum: float = 0.95, nesterov: bool = True, rms: float = 0.2,
+                 ns_steps: int = 5, ns_coefficients=muon_ops.COEFFICIENTS, betas=(0.9, 0.95), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, capturable: bool = False):
+        if not 0 <= momentum < 1 or not rms > 0 or ns_steps < 1 or len(ns_coefficients) != 3:
+            raise ValueError("invalid Muon hyper-parameters")
+        # add_param_group (called by the base constructor) completes each group from these
+        self._matrix_defaults = dict(momentum=momentum, nesterov=nesterov, rms=rms, ns_steps=ns_steps,
+                                     ns_coefficients=tuple(ns_coefficients))
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable)
+
+    def add_param_group(self, group: dict) -> None:
+        params = group["params"]
+        group["params"] = params = [params] if isinstance(params, torch.Tensor) else list(params)
+        matrices = [p.dim() == 2 and p.dtype == torch.float32 for p in params]
+        group.setdefault("orthogonal", all(matrices))
+        if group["orthogonal"]:
+            if not all(matrices):
+                bad = next(p for p, ok in zip(params, matrices) if not ok)
+                raise ValueError(f"Muon: a {tuple(bad.shape)} {bad.dtype} parameter is not a float32 matrix; put it in a "
+                                 "group with orthogonal=False")
+            for k, v in self._matrix_defaults.items():
+                group.setdefault(k, v)
+        super().add_param_group(group)
+
+    def _orthogonal_step(self, gi, group, params, inv_scale, skip) -> None:
+        from .models.fused_gpt import _SHADOW, _SHADOW_VER
+
+        self._wait_for(params)
+        lr = group["lr"]
+        cuda = params[0].is_cuda
+        if self.capturable and cuda:
+            capturing = torch.cuda.is_current_stream_capturing()
+            if gi not in self._hp:
+                if capturing:
+                    raise RuntimeError("Muon(capturable=True) needs one eager step before capture")
+                self._hp[gi] = torch.tensor([lr, 0.0], dtype=torch.float32, device=params[0].device)
+                self._hp_lr[gi] = float(lr)
+            if not capturing:
+                self.sync_hyperparams()
+            lr = self._hp[gi][:1]
+        todo = [p for p in params if not self.state[p]]
+        if todo:
+            flat = torch.zeros(sum((p.numel() + 3) // 4 * 4 for p in todo), dtype=torch.float32, device=todo[0].device)
+            off = 0
+            for p in todo:
+                self.state[p]["momentum_buffer"] = flat[off: off + p.numel()].view_as(p)
+                off += (p.numel() + 3) // 4 * 4
+        shadows = None
+        if cuda:  # the bf16 copies that are up to date stay so; others are cast by the next forward
+            shadows = [getattr(p, _SHADOW, None) for p in params]
+            shadows = [sh if sh is not None and sh.shape == p.shape and getattr(p, _SHADOW_VER, None) == p._version
+                       else None for p, sh in zip(params, shadows)]
+        muon_ops.muon_update_(params, [p.grad.float() for p in params],
+                              [self.state[p]["momentum_buffer"] for p in params], lr=lr, momentum=group["momentum"],
+                              nesterov=group["nesterov"], weight_decay=group["weight_decay"], steps=group["ns_steps"],
+                              coefficients=group["ns_coefficients"], rms=group["rms"], shadows=shadows,
+                              inv_scale=inv_scale, skip=skip)
+        if cuda:
+            self._ensure_grad_buffers()
+
+
+def muon_groups(model: torch.nn.Module, weight_decay: float | None = None) -> list[dict]:
+    """``model``'s parameters as Muon's groups: the matrices of its blocks, and (``orthogonal=False``) the
+    embeddings, the LM head and everything that is not a matrix.  ``weight_decay`` applies to matrices
+    of both groups; biases and norms, a group of their own, then take none."""
+    hidden, tables, small = [], [], []
+    for name, p in model.named_parameters():
+        if not p.requires_grad:
+            continue
+        outer = any(part in ("wte", "wpe", "head", "embedding", "lm_head") for part in name.split("."))
+        (small if p.dim() < 2 else tables if outer or p.dim() != 2 else hidden).append(p)
+    groups = [dict(params=hidden, orthogonal=True), dict(params=tables, orthogonal=False),
+              dict(params=small, orthogonal=False)]
+    if weight_decay is not None:
+        groups[0]["weight_decay"] = groups[1]["weight_decay"] = weight_decay
+        groups[2]["weight_decay"] = 0.0
+    return [g for g in groups if g["params"]]

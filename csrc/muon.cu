@@ -28,7 +28,9 @@
 // One persistent warp-specialised kernel does every product: TMA loads, one
 // tcgen05.mma issuer, accumulators double-buffered in TMEM so that a tile's
 // epilogue runs under the next one's products.  A tile is 256 x 256 on a pair
-// of SMs (cta_group::2) or 128 x 128 on one.
+// of SMs (cta_group::2) or 128 x 128 on one; where there are fewer of those than
+// SMs, a cluster shares the K of each and adds the parts up over distributed
+// shared memory.
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
@@ -96,11 +98,12 @@ template <typename T, bool STEP>
 __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ MdMuonParams p, float* __restrict__ partial) {
   pdl_trigger();
   pdl_wait();
+  const int which = blockIdx.y;
   const long long n = static_cast<long long>(p.rows) * p.cols;
   const long long lo = static_cast<long long>(blockIdx.x) * kChunk;
   const long long hi = lo + kChunk < n ? lo + kChunk : n;
-  const T* g = static_cast<const T*>(p.src[blockIdx.y]);
-  float* m = p.m[blockIdx.y];
+  const T* g = static_cast<const T*>(p.src[which]);
+  float* m = p.m[which];
   if (STEP && p.skip != nullptr && *p.skip != 0.f) return;
   const float gs = STEP && p.inv_scale != nullptr ? *p.inv_scale : 1.f;
   float sum = 0.f;
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
     if (STEP) m[k] = mv;
   }
   sum = block_sum(sum);
-  if (threadIdx.x == 0) partial[static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x] = sum;
+  if (threadIdx.x == 0) partial[static_cast<long long>(which) * gridDim.x + blockIdx.x] = sum;
 }
 
 __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
@@ -146,22 +149,23 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
                                                            __half* __restrict__ xl, int ldx) {
   pdl_trigger();
   pdl_wait();
+  const int which = blockIdx.y;
   // The chunks' shares in a fixed order (the same in every block of the matrix).
   float total = 0.f;
   for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += kThreads)
-    total += partial[static_cast<long long>(blockIdx.y) * gridDim.x + i];
+    total += partial[static_cast<long long>(which) * gridDim.x + i];
   total = block_sum(total);
   const float inv = kScale / (sqrtf(total) + p.eps);
   const long long n = static_cast<long long>(p.rows) * p.cols;
   const long long lo = static_cast<long long>(blockIdx.x) * kChunk;
   const long long hi = lo + kChunk < n ? lo + kChunk : n;
-  const T* g = static_cast<const T*>(p.src[blockIdx.y]);
-  const float* m = p.m[blockIdx.y];
+  const T* g = static_cast<const T*>(p.src[which]);
+  const float* m = p.m[which];
   const float gs = STEP && p.inv_scale != nullptr ? *p.inv_scale : 1.f;
   // Position of the chunk's first element; inside the chunk 32-bit division is enough.
   const long long row_lo = lo / p.cols;
   const uint32_t col_lo = static_cast<uint32_t>(lo - row_lo * p.cols), cols = static_cast<uint32_t>(p.cols);
-  const long long base = (static_cast<long long>(blockIdx.y) * p.rows + row_lo) * ldx;
+  const long long base = (static_cast<long long>(which) * p.rows + row_lo) * ldx;
   auto place = [&](uint32_t i) {  // of element lo + i
     const uint32_t e = col_lo + i, r = e / cols;
     return base + static_cast<long long>(r) * ldx + (e - r * cols);
@@ -202,6 +206,9 @@ constexpr int kStages = 5;
 constexpr int kEpiWarps = 8;
 constexpr int kChunkBytes = 32 * 32 * 2;       // an epilogue chunk of fp16: 32 rows x 64 bytes
 constexpr int kWarpBytes = 4 * kChunkBytes;    // a warp's staging
+constexpr int kSplitStages = 3;                // K shared by a cluster: fewer stages, and 64 KB for
+constexpr int kPartBytes = 32 * 32 * 4;        // the partial sums of its chunks
+static_assert(2 * kSplitStages * kOperand + 16 * kPartBytes <= 2 * kStages * kOperand, "partial sums");
 constexpr int kSmemBytes = 1024 + kStages * 2 * kOperand + kEpiWarps * kWarpBytes + 512;
 constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
 
@@ -214,7 +221,7 @@ enum Mode : int { kGram = 0, kPoly = 1, kNext = 2, kLast = 3 };
 
 struct GemmParams {
   int M, N, K;
-  int tiles_m, tiles_n, per_batch, units, k_blocks;
+  int tiles_m, tiles_n, per_batch, units, k_blocks, splits;
   float alpha, beta;
   // kLast: what leaves
   int dtype, step;
@@ -244,6 +251,12 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t smem_addr, uint32_t cta)
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// By every warp, its lanes together again: what was written to the others' shared memory is there.
+__device__ __forceinline__ void cluster_join() {
+  __syncwarp();
+  cluster_sync();
 }
 
 // Tile load whose bytes are counted on `bar`: this CTA's barrier, or with CG = 2 the pair
@@ -463,39 +476,61 @@ __device__ __forceinline__ void write_out(const GemmParams& p, const Out& o, uin
   }
 }
 
+// 32 x 32 fp32 in 128-byte rows, 16-byte pieces swizzled by the row: the lane's row in and out.
+__device__ __forceinline__ void put_staged(uint32_t staged, int lane, const float (&v)[32]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(staged + lane * 128 + ((q ^ (lane & 7)) << 4)),
+                 "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
+                 : "memory");
+}
+__device__ __forceinline__ void get_staged(uint32_t staged, int lane, float (&v)[32]) {
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v[4 * q]), "=f"(v[4 * q + 1]), "=f"(v[4 * q + 2]), "=f"(v[4 * q + 3])
+                 : "r"(staged + lane * 128 + ((q ^ (lane & 7)) << 4))
+                 : "memory");
+}
+
 struct Maps {
   CUtensorMap a[2], b[2], c[2], d[2];  // high and low parts: operands, addend, result
 };
 
-template <int CG, bool SPLIT, bool A_MN, bool B_MN, int MODE>
+// KS (CG = 1): the blocks of K are shared by a cluster of `splits` CTAs, which sum their accumulators over
+// distributed shared memory and finish a share of the tile each.
+template <int CG, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmParams p) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
   constexpr int BN = BM * CG;  // tile columns (and rows of the pair's tile)
   constexpr int kTmemCols = 2 * BN;
+  constexpr int kSt = KS ? kSplitStages : kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = smem + kStages * kOperand;
+  uint8_t* sB = smem + kSt * kOperand;
+  uint8_t* sRed = smem + 2 * kSplitStages * kOperand;  // KS: 16 chunks of partial sums per CTA of the cluster
   uint8_t* sEpi = smem + 2 * kStages * kOperand;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + kEpiWarps * kWarpBytes);
   uint64_t* full_bar = bars;
-  uint64_t* empty_bar = bars + kStages;
-  uint64_t* tfull_bar = bars + 2 * kStages;
-  uint64_t* tempty_bar = bars + 2 * kStages + 2;
-  uint64_t* drain_bar = bars + 2 * kStages + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 5);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * kStages + 6);
-  uint64_t* c_bar = bars + 2 * kStages + 7;  // two per epilogue warp
+  uint64_t* empty_bar = bars + kSt;
+  uint64_t* tfull_bar = bars + 2 * kSt;
+  uint64_t* tempty_bar = bars + 2 * kSt + 2;
+  uint64_t* drain_bar = bars + 2 * kSt + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kSt + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * kSt + 6);
+  uint64_t* c_bar = bars + 2 * kSt + 7;  // two per epilogue warp
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = CG == 2 ? cluster_ctarank() : 0u;
+  const int part = KS ? static_cast<int>(cluster_ctarank()) : 0;
   const bool leader = crank == 0;
-  const int first = CG == 2 ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
-  const int stride = CG == 2 ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  const int group = KS ? p.splits : CG;  // CTAs that share a tile
+  const int first = static_cast<int>(blockIdx.x) / group, stride = static_cast<int>(gridDim.x) / group;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < kSt; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
@@ -522,27 +557,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync();  // the peer's barriers exist before anything arrives on them
+  if constexpr (CG == 2 || KS) cluster_sync();  // the others run, and their barriers exist, before anything reaches them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   pdl_trigger();
   pdl_wait();
 
   const int blocks = p.k_blocks * (SPLIT ? 3 : 1);
+  const int lo = KS ? blocks * part / p.splits : 0, hi = KS ? blocks * (part + 1) / p.splits : blocks;
   const int run = SPLIT ? kSplitRun : blocks;  // blocks that one accumulator adds up
+  // A tile on the diagonal of X X^T or A A: both operands are the same rows, loaded once.
+  auto same = [&](int tm, int tn, int i) { return SYM && tm == tn && i < p.k_blocks; };
   if (warp == 0 && lane == 0) {
     // ---------------------------------------------------------- producer
     int stage = 0;
     uint32_t phase = 0;
-    int armed[kStages];
-    for (int s = 0; s < kStages; ++s) armed[s] = -1;
+    int armed[kSt];
+    for (int s = 0; s < kSt; ++s) armed[s] = -1;
     bool ok = true;
     for (int u = first; u < p.units && ok; u += stride) {
       int b, tm, tn;
       decode<SYM>(p, u, b, tm, tn);
       const int row = tm * (CG * BM) + static_cast<int>(crank) * BM;
       const int col = tn * BN + static_cast<int>(crank) * BM;
-      for (int i = 0; i < blocks; ++i) {
+      for (int i = lo; i < hi; ++i) {
         // high x high, high x low, low x high
         const int which = i / p.k_blocks, k = (i - which * p.k_blocks) * BK;
         const CUtensorMap* ta = &maps.a[which == 2];
@@ -553,7 +591,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         uint32_t bar = smem_u32(&full_bar[stage]);
         if constexpr (CG == 2) bar = map_to_cta(bar, 0);
-        if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * 2 * kOperand);
+        const bool once = same(tm, tn, i);
+        if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * (once ? 1 : 2) * kOperand);
         armed[stage] = static_cast<int>(phase);
         uint8_t* da = sA + stage * kOperand;
         uint8_t* db = sB + stage * kOperand;
@@ -563,13 +602,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         } else {
           load_tile<CG>(ta, bar, da, k, row, b);
         }
-        if (B_MN) {
+        if (once) {
+        } else if (B_MN) {
           load_tile<CG>(tb, bar, db, col, k, b);
           load_tile<CG>(tb, bar, db + kOperand / 2, col + 64, k, b);
         } else {
           load_tile<CG>(tb, bar, db, k, col, b);
         }
-        if (++stage == kStages) {
+        if (++stage == kSt) {
           stage = 0;
           phase ^= 1u;
         }
@@ -578,7 +618,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // No copy into this pair's shared memory may be in flight at exit (the follower's are counted
     // on the leader's barriers, which the leader's MMA has consumed before the last cluster barrier).
     if (leader)
-      for (int s = 0; s < kStages; ++s)
+      for (int s = 0; s < kSt; ++s)
         if (armed[s] >= 0) mbar_wait(&full_bar[s], static_cast<uint32_t>(armed[s]), p.status, 421, nullptr);
   } else if (warp == 1 && leader) {
     // ---------------------------------------------------------- MMA issuer
@@ -590,14 +630,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
     for (int u = first; u < p.units && ok; u += stride) {
-      for (int i0 = 0; i0 < blocks; i0 += run) {
+      int b, tm, tn;
+      decode<SYM>(p, u, b, tm, tn);
+      for (int i0 = lo; i0 < hi; i0 += run) {
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.status, 422, abort_flag)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-        const int i1 = min(blocks, i0 + run);
+        const int i1 = min(hi, i0 + run);
         for (int i = i0; i < i1; ++i) {
           if (!mbar_wait(&full_bar[stage], phase, p.status, 423, abort_flag)) {
             ok = false;
@@ -605,13 +647,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
           tc_fence_after();
           const uint64_t a_st = a_base + static_cast<uint32_t>(stage * kOperand >> 4);
-          const uint64_t b_st = b_base + static_cast<uint32_t>(stage * kOperand >> 4);
+          const uint64_t b_st = (same(tm, tn, i) ? a_base : b_base) + static_cast<uint32_t>(stage * kOperand >> 4);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
             mma<CG>(d_tmem, a_st + (A_MN ? k * (2048 >> 4) : k * (32 >> 4)), b_st + (B_MN ? k * (2048 >> 4) : k * (32 >> 4)),
                     idesc, (i > i0 || k > 0) ? 1u : 0u);
           commit_all<CG>(&empty_bar[stage]);
-          if (++stage == kStages) {
+          if (++stage == kSt) {
             stage = 0;
             phase ^= 1u;
           }
@@ -682,136 +724,205 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       }
     };
     bool ok = true;
-    for (int u = first; u < p.units && ok; u += stride) {
-      int b, tm, tn;
-      decode<SYM>(p, u, b, tm, tn);
-      const int row0 = tm * (CG * BM) + static_cast<int>(crank) * BM + quarter * 32;
-      const int col0 = tn * BN + half * kChunks * 32;
-      // This warp's chunks: up to the last column, or the one that holds the diagonal.
-      const int end = SYM ? min(p.N, row0 + 32) : p.N;
-      const int chunks = row0 < p.M && end > col0 ? min(kChunks, (end - col0 + 31) / 32) : 0;
-      if (kAddend && chunks > 0) fetch(ctr, b, row0, col0);
-      Out out;
-      float4 old[8];
-      if constexpr (MODE == kLast) {
-        const float lr = p.lr != nullptr ? *p.lr : 1.f;
-        out.rate = p.step ? -p.rate * lr * (1.f / kScale) : 1.f / kScale;
-        out.decay = p.lr != nullptr ? 1.f - lr * p.decay : p.decay;
-        out.idle = p.step && p.skip != nullptr && *p.skip != 0.f;
-        const unsigned long long piece = p.dtype == 2 ? 15u : 7u;
-        out.wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out[b]) & piece) == 0 &&
-                   (reinterpret_cast<uintptr_t>(p.shadow[b]) & 7u) == 0;
-        if (chunks > 0) load_old(p, out, b, row0, col0, lane, old);
-      }
-      float sum[SPLIT ? kChunks * 32 : 1];
-      if constexpr (SPLIT) {
+    Out out;
+    float4 old[8];
+    auto prepare_out = [&](int b, int row0, int n0) {
+      const float lr = p.lr != nullptr ? *p.lr : 1.f;
+      out.rate = p.step ? -p.rate * lr * (1.f / kScale) : 1.f / kScale;
+      out.decay = p.lr != nullptr ? 1.f - lr * p.decay : p.decay;
+      out.idle = p.step && p.skip != nullptr && *p.skip != 0.f;
+      const unsigned long long piece = p.dtype == 2 ? 15u : 7u;
+      out.wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out[b]) & piece) == 0 &&
+                 (reinterpret_cast<uintptr_t>(p.shadow[b]) & 7u) == 0;
+      load_old(p, out, b, row0, n0, lane, old);
+    };
+    auto load_acc = [&](int c, float (&v)[32]) {  // this warp's chunk c of the current accumulator
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(acc * BN + (half * kChunks + c) * 32), r);
+      tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < kChunks * 32; ++j) sum[j] = 0.f;
-        for (int i0 = 0; i0 < blocks && ok; i0 += run) {
-          if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) {
-            ok = false;
-            break;
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+    };
+    // Split products: the runs of this warp's columns, added up in registers.
+    auto add_runs = [&](float (&sum)[kChunks * 32]) {
+#pragma unroll
+      for (int j = 0; j < kChunks * 32; ++j) sum[j] = 0.f;
+      for (int i0 = lo; i0 < hi; i0 += run) {
+        if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) {
+          ok = false;
+          return;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          float v[32];
+          load_acc(c, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sum[c * 32 + j] += v[j];
+        }
+        release();
+      }
+    };
+    // A chunk of products, from here to memory.  `more`: another one of this tile follows on its right.
+    auto finish = [&](float (&v)[32], int b, int row0, int n0, bool more) {
+      const uint32_t slot = base + (ctr % kSlots) * (kWarpBytes / 2);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= p.alpha;
+      if constexpr (kAddend) {
+        if (kSlots == 2 && more) fetch(ctr + 1, b, row0, n0 + 32);
+        if (!mbar_wait(&cb[ctr % kSlots], static_cast<uint32_t>(ctr / kSlots) & 1u, p.status, 426, abort_flag)) {
+          ok = false;
+          return;
+        }
+        add_staged(slot, lane, p.beta, v);
+        if (kAddLow) add_staged(slot + kChunkBytes, lane, p.beta, v);
+        --coming;
+        __syncwarp();  // the whole chunk has been read
+      } else {
+        // (the other slot's result may still be leaving; this one's has to be out)
+        if (lane == 0) {
+          if (kSlots == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          else bulk_wait_read_all();
+        }
+        __syncwarp();
+      }
+      if constexpr (MODE == kLast) {
+        put_staged(slot, lane, v);
+        __syncwarp();
+        write_out(p, out, slot, b, row0, n0, lane, old);
+        if (more) load_old(p, out, b, row0, n0 + 32, lane, old);
+      } else {
+        const bool mirrored = SYM && n0 < row0;  // (the block on the diagonal is its own mirror image)
+        uint32_t h[16], l[16];
+        split32<kLow>(v, h, l);
+        stage(slot, lane, h);
+        if (kLow) stage(slot + kChunkBytes, lane, l);
+        constexpr uint32_t kMirror = kLow ? 2 * kChunkBytes : kChunkBytes;
+        if (SYM && mirrored) {
+          stage_mirrored(slot + kMirror, lane, h);
+          if (kLow) stage_mirrored(slot + kMirror + kChunkBytes, lane, l);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d_at(&maps.d[0], slot, n0, row0, b);
+          if (kLow) tma_store_3d_at(&maps.d[1], slot + kChunkBytes, n0, row0, b);
+          if (SYM && mirrored) {
+            tma_store_3d_at(&maps.d[0], slot + kMirror, row0, n0, b);
+            if (kLow) tma_store_3d_at(&maps.d[1], slot + kMirror + kChunkBytes, row0, n0, b);
           }
-          tc_fence_after();
+          bulk_commit_group();
+        }
+      }
+      ++ctr;
+      if (kAddend && kSlots == 1 && more) fetch(ctr, b, row0, n0 + 32);
+    };
+    // Whether the 32 x 32 chunk at (row0, n0) is to be computed.
+    auto wanted = [&](int row0, int n0) { return row0 < p.M && n0 < p.N && (!SYM || n0 <= row0); };
+
+    if constexpr (KS) {
+      // The tile's 16 chunks are dealt to the CTAs: chunk t (columns t / 4, rows t % 4) belongs to CTA
+      // t / per, warp t % per there.
+      int b, tm, tn;
+      decode<SYM>(p, first, b, tm, tn);
+      const int per = 16 / p.splits, mine = part * per + (warp - 2);
+      const int row0 = tm * BM + (mine & 3) * 32, n0 = tn * BN + (mine >> 2) * 32;
+      const bool has = warp - 2 < per && wanted(row0, n0);
+      if (kAddend && has) fetch(ctr, b, row0, n0);
+      if constexpr (MODE == kLast)
+        if (has) prepare_out(b, row0, n0);
+      auto send = [&](int c, float (&v)[32]) {
+        const int column = half * kChunks + c, t = column * 4 + quarter;
+        if (!wanted(tm * BM + quarter * 32, tn * BN + column * 32)) return;
+        const uint32_t to = map_to_cta(smem_u32(sRed) + ((t % per) * p.splits + part) * kPartBytes, t / per);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + lane * 128 + ((q ^ (lane & 7)) << 4)),
+                       "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
+                       : "memory");
+      };
+      if constexpr (SPLIT) {
+        float sum[kChunks * 32];
+        add_runs(sum);
+        if (ok) {
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                   static_cast<uint32_t>(acc * BN + (half * kChunks + c) * 32), r);
-            tmem_ld_wait();
+            float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c * 32 + j] += __uint_as_float(r[j]);
+            for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j];
+            send(c, v);
+          }
+        }
+      } else {
+        ok = mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag);
+        if (ok) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < kChunks; ++c) {
+            float v[32];
+            load_acc(c, v);
+            send(c, v);
+          }
+        }
+      }
+      cluster_join();
+      if (ok && has) {
+        float v[32];
+        const uint32_t from = smem_u32(sRed) + (warp - 2) * p.splits * kPartBytes;
+        get_staged(from, lane, v);
+#pragma unroll 1
+        for (int s = 1; s < p.splits; ++s) {
+          float w[32];
+          get_staged(from + s * kPartBytes, lane, w);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += w[j];
+        }
+        finish(v, b, row0, n0, false);
+      }
+    } else {
+      for (int u = first; u < p.units && ok; u += stride) {
+        int b, tm, tn;
+        decode<SYM>(p, u, b, tm, tn);
+        const int row0 = tm * (CG * BM) + static_cast<int>(crank) * BM + quarter * 32;
+        const int col0 = tn * BN + half * kChunks * 32;
+        int chunks = 0;  // (those wanted come first)
+        while (chunks < kChunks && wanted(row0, col0 + chunks * 32)) ++chunks;
+        if (kAddend && chunks > 0) fetch(ctr, b, row0, col0);
+        if constexpr (MODE == kLast)
+          if (chunks > 0) prepare_out(b, row0, col0);
+        if constexpr (SPLIT) {
+          float sum[kChunks * 32];
+          add_runs(sum);
+          // (unrolled, so that the sums stay in registers)
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c)
+            if (c < chunks && ok) {
+              float v[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j];
+              finish(v, b, row0, col0 + c * 32, c + 1 < chunks);
+            }
+        } else {
+          if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < chunks && ok; ++c) {
+            float v[32];
+            load_acc(c, v);
+            finish(v, b, row0, col0 + c * 32, c + 1 < chunks);
           }
           release();
         }
-        if (!ok) break;
-      } else {
-        if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) break;
-        tc_fence_after();
       }
-      auto chunk = [&](int c) {
-        const int n0 = col0 + c * 32;
-        const uint32_t slot = base + (ctr % kSlots) * (kWarpBytes / 2);
-        float v[32];
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = sum[c * 32 + j] * p.alpha;
-        } else {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                                 static_cast<uint32_t>(acc * BN + (half * kChunks + c) * 32), r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * p.alpha;
-        }
-        if constexpr (kAddend) {
-          if (kSlots == 2 && c + 1 < chunks) fetch(ctr + 1, b, row0, n0 + 32);
-          if (!mbar_wait(&cb[ctr % kSlots], static_cast<uint32_t>(ctr / kSlots) & 1u, p.status, 426, abort_flag)) {
-            ok = false;
-            return;
-          }
-          add_staged(slot, lane, p.beta, v);
-          if (kAddLow) add_staged(slot + kChunkBytes, lane, p.beta, v);
-          --coming;
-          __syncwarp();  // the whole chunk has been read
-        } else {
-          // (the other slot's result may still be leaving; this one's has to be out)
-          if (lane == 0) {
-            if (kSlots == 2) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-            else bulk_wait_read_all();
-          }
-          __syncwarp();
-        }
-        if constexpr (MODE == kLast) {
-#pragma unroll
-          for (int q = 0; q < 8; ++q)
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(slot + lane * 128 + ((q ^ (lane & 7)) << 4)),
-                         "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
-                         : "memory");
-          __syncwarp();
-          write_out(p, out, slot, b, row0, n0, lane, old);
-          if (c + 1 < chunks) load_old(p, out, b, row0, n0 + 32, lane, old);
-        } else {
-          const bool mirrored = SYM && n0 < row0;  // (the block on the diagonal is its own mirror image)
-          uint32_t h[16], l[16];
-          split32<kLow>(v, h, l);
-          stage(slot, lane, h);
-          if (kLow) stage(slot + kChunkBytes, lane, l);
-          constexpr uint32_t kMirror = kLow ? 2 * kChunkBytes : kChunkBytes;
-          if (SYM && mirrored) {
-            stage_mirrored(slot + kMirror, lane, h);
-            if (kLow) stage_mirrored(slot + kMirror + kChunkBytes, lane, l);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_3d_at(&maps.d[0], slot, n0, row0, b);
-            if (kLow) tma_store_3d_at(&maps.d[1], slot + kChunkBytes, n0, row0, b);
-            if (SYM && mirrored) {
-              tma_store_3d_at(&maps.d[0], slot + kMirror, row0, n0, b);
-              if (kLow) tma_store_3d_at(&maps.d[1], slot + kMirror + kChunkBytes, row0, n0, b);
-            }
-            bulk_commit_group();
-          }
-        }
-        ++ctr;
-        if (kAddend && kSlots == 1 && c + 1 < chunks) fetch(ctr, b, row0, n0 + 32);
-      };
-      if constexpr (SPLIT) {  // (unrolled, so that the sums stay in registers)
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-          if (c < chunks && ok) chunk(c);
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < chunks && ok; ++c) chunk(c);
-      }
-      if constexpr (!SPLIT) release();
     }
     // Nothing may be in flight into or out of shared memory at exit.
     for (; coming > 0; --coming, ++ctr)
       mbar_wait(&cb[ctr % kSlots], static_cast<uint32_t>(ctr / kSlots) & 1u, p.status, 427, nullptr);
     if (lane == 0) bulk_wait_all();
   }
+  if constexpr (KS)
+    if (warp < 2) cluster_join();
   tc_fence_before();
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();
@@ -876,7 +987,7 @@ int sms() {
   return n;
 }
 
-template <int CG, bool SPLIT, bool A_MN, bool B_MN, int MODE>
+template <int CG, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
 cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p, int count,
                            cudaStream_t stream) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
@@ -886,7 +997,7 @@ cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pa
   p.per_batch = SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
   p.units = p.per_batch * count;
   p.k_blocks = (p.K + BK - 1) / BK;
-  auto kern = product_kernel<CG, SPLIT, A_MN, B_MN, MODE>;
+  auto kern = product_kernel<CG, KS, SPLIT, A_MN, B_MN, MODE>;
   static int done[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -895,18 +1006,18 @@ cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pa
     if (e != cudaSuccess) return e;
     if (dev < 64) done[dev] = 1;
   }
-  const int slots = sms() / CG;
+  const int slots = sms() / CG, group = KS ? p.splits : CG;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(CG * (p.units < slots ? p.units : slots)));
+  cfg.gridDim = dim3(static_cast<unsigned>(group * (KS || p.units < slots ? p.units : slots)));
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
   cfg.numAttrs = 0;
-  if (CG == 2) {
+  if (CG == 2 || KS) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = 2;
+    attr[cfg.numAttrs].val.clusterDim.x = group;
     attr[cfg.numAttrs].val.clusterDim.y = 1;
     attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
@@ -926,12 +1037,28 @@ cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pa
   return cudaLaunchKernelEx(&cfg, kern, maps, p);
 }
 
+// How a product is cut.  `tile`: 0 choose, 1: 128 x 128 tiles, 2: 256 x 256 tiles on SM pairs.
 template <bool A_MN, bool B_MN, int MODE>
 cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p,
                     int count, cudaStream_t s) {
-  if (split) return launch_product<1, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
-  return tile == 2 ? launch_product<2, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)
-                   : launch_product<1, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  constexpr bool SYM = MODE == kGram || MODE == kPoly;
+  auto units = [&](int t) {
+    const long long m = (p.M + t - 1) / t, n = (p.N + t - 1) / t;
+    return (SYM ? m * (m + 1) / 2 : m * n) * count;
+  };
+  // Few tiles: K is shared by as many CTAs as fit the SMs together and keep four blocks each.
+  const int blocks = (p.K + BK - 1) / BK * (split ? 3 : 1);
+  p.splits = 1;
+  if (tile == 0)
+    while (p.splits < 8 && units(BM) * 2 * p.splits <= sms() && blocks >= 8 * p.splits) p.splits *= 2;
+  if (p.splits > 1)
+    return split ? launch_product<1, true, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)
+                 : launch_product<1, true, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  if (split) return launch_product<1, false, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  // Pairs of SMs where their larger tiles still occupy half of the SMs.
+  if (tile == 2 || (tile == 0 && units(2 * BM) >= sms() / 4))
+    return launch_product<2, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  return launch_product<1, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
 }
 
 struct Layout {  // byte offsets in the workspace (each 256-byte aligned)
@@ -1014,13 +1141,6 @@ extern "C" int md_muon(const MdMuonParams* prm, cudaStream_t stream) {
                                    : prepare<float, false>(p, l, static_cast<int>(chunks), stream);
   if (e != cudaSuccess) return static_cast<int>(e);
 
-  // Pairs of SMs where their larger tiles still occupy most of the SMs.
-  const auto tiles = [](long long n, int t) { return (n + t - 1) / t; };
-  const long long sym = tiles(small, 256) * (tiles(small, 256) + 1) / 2 * p.count;
-  const long long all = tiles(p.rows, 256) * tiles(p.cols, 256) * p.count;
-  const int tile_sym = p.tile ? p.tile : (sym >= sms() / 4 ? 2 : 1);
-  const int tile_all = p.tile ? p.tile : (all >= sms() / 4 ? 2 : 1);
-
   GemmParams g{};
   g.status = p.status;
   g.dtype = p.dtype, g.step = p.step;
@@ -1033,23 +1153,23 @@ extern "C" int md_muon(const MdMuonParams* prm, cudaStream_t stream) {
     // A = X X^T (X^T X)
     g.M = g.N = small, g.K = tall ? p.rows : p.cols;
     g.alpha = per, g.beta = 0.f;
-    e = tall ? product<true, true, kGram>(tile_sym, split, xs, xs, a, a, g, p.count, stream)
-             : product<false, false, kGram>(tile_sym, split, xs, xs, a, a, g, p.count, stream);
+    e = tall ? product<true, true, kGram>(p.tile, split, xs, xs, a, a, g, p.count, stream)
+             : product<false, false, kGram>(p.tile, split, xs, xs, a, a, g, p.count, stream);
     if (e != cudaSuccess) break;
     // B = b A + c A A
     g.K = small;
     g.alpha = p.c * per, g.beta = p.b;
-    e = product<false, false, kPoly>(tile_sym, split, a, a, a, f, g, p.count, stream);
+    e = product<false, false, kPoly>(p.tile, split, a, a, a, f, g, p.count, stream);
     if (e != cudaSuccess) break;
     // X <- a X + B X (X B)
     g.M = p.rows, g.N = p.cols;
     g.alpha = per, g.beta = p.a;
     if (last)
-      e = tall ? product<false, false, kLast>(tile_all, split, xs, f, xs, xn, g, p.count, stream)
-               : product<false, true, kLast>(tile_all, split, f, xs, xs, xn, g, p.count, stream);
+      e = tall ? product<false, false, kLast>(p.tile, split, xs, f, xs, xn, g, p.count, stream)
+               : product<false, true, kLast>(p.tile, split, f, xs, xs, xn, g, p.count, stream);
     else
-      e = tall ? product<false, false, kNext>(tile_all, split, xs, f, xs, xn, g, p.count, stream)
-               : product<false, true, kNext>(tile_all, split, f, xs, xs, xn, g, p.count, stream);
+      e = tall ? product<false, false, kNext>(p.tile, split, xs, f, xs, xn, g, p.count, stream)
+               : product<false, true, kNext>(p.tile, split, f, xs, xs, xn, g, p.count, stream);
   }
   return static_cast<int>(e);
 }

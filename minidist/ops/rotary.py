@@ -130,9 +130,13 @@ def _turn(q, k, table, positions, interleaved, inverse, inplace=False):
     if inplace:
         q_out, k_out = q, k
     else:
-        q, k = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (q, k))
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+        if q.stride(-1) != 1:
+            q = q.contiguous()
+        q_out, k_out = torch.empty_like(q, memory_format=torch.contiguous_format), None
+        if k is not None:
+            if k.stride(-1) != 1:
+                k = k.contiguous()
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     _launch(q, k, q_out, k_out, table, positions, interleaved, inverse)
     return [q_out, k_out]
 

@@ -31,6 +31,15 @@
 // of SMs (cta_group::2) or 128 x 128 on one; where there are fewer of those than
 // SMs, a cluster shares the K of each and adds the parts up over distributed
 // shared memory.
+//
+// Measured (B200; cuBLAS bf16 1634 TFLOP/s in bursts, 1395 sustained under the
+// power cap), useful operations, symmetric ones counted once: 4096 x 4096, five
+// steps, 1.16 ms = 1190 TFLOP/s in bursts, 1.39 ms = 990 sustained (tensor pipe
+// active 69 to 78 % of the time; the rest is the last wave of 256 tiles on 74
+// pairs).  12 x 2304 x 768 with momentum and weights 490 us = 555 TFLOP/s: K is 768,
+// so a tile brings 512 KB of addend and result to 768 KB of operands (measured
+// without them: 420 us).  768 x 768 128 us: 17 launches of 7.5 us, each a chain of
+// launch, first load, 12 blocks of K and epilogue, on 21 to 72 of the SMs.
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 

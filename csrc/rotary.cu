@@ -20,6 +20,14 @@
 // four heads: cos and sin are loaded once for all four, the index arithmetic
 // (multiplications instead of divisions) is paid once, and the channels that pass
 // through are copied by the same threads in vectors of their own width.
+//
+// Measured (B200, copy rate 6.55 TB/s): 20011 tokens of 32 + 32 heads of 80, 40 of
+// them turned, bf16: 74 us, 5.5 TB/s (a loop over vectors with divisions and single
+// conversions: 190 us, of which 45 % was issuing instructions); 16 x 1024 tokens of
+// 12 + 12 heads of 64 in a packed projection: 20 us, 5.0 TB/s, a third of it start
+// and end of so short a launch; fp32 heads of 128: 6.4 TB/s; one token for each of
+// 32 sequences: 1.9 us.  Two heads per thread instead of four measured the same
+// within 5 % on paired layouts and 15 % slower on interleaved ones.
 #include <cuda_fp16.h>
 
 #include <type_traits>

@@ -28,9 +28,9 @@
 // One persistent warp-specialised kernel does every product: TMA loads, one
 // tcgen05.mma issuer, accumulators double-buffered in TMEM so that a tile's
 // epilogue runs under the next one's products.  A tile is 256 x 256 on a pair
-// of SMs (cta_group::2) or 128 x 128 on one; where there are fewer of those than
-// SMs, a cluster shares the K of each and adds the parts up over distributed
-// shared memory.
+// of SMs (cta_group::2), 128 x 128 on one or, where that leaves SMs idle, 128 x 64;
+// where SMs are idle all the same, a cluster shares the K of each tile and adds
+// the parts up over distributed shared memory.
 //
 // Measured (B200; cuBLAS bf16 1634 TFLOP/s in bursts, 1395 sustained under the
 // power cap), useful operations, symmetric ones counted once: 4096 x 4096, five
@@ -208,17 +208,15 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
 // ---------------------------------------------------------------------------
 // The products
 // ---------------------------------------------------------------------------
-constexpr int BM = 128;   // rows of A and of B per CTA and stage
+constexpr int BM = 128;   // rows of A per CTA and stage
 constexpr int BK = 64;
 constexpr int kOperand = BM * BK * 2;  // 16 KB
-constexpr int kStages = 5;
+constexpr int kRing = 10 * kOperand;   // shared memory for the stages (and the partial sums of a shared K)
 constexpr int kEpiWarps = 8;
 constexpr int kChunkBytes = 32 * 32 * 2;       // an epilogue chunk of fp16: 32 rows x 64 bytes
 constexpr int kWarpBytes = 4 * kChunkBytes;    // a warp's staging
-constexpr int kSplitStages = 3;                // K shared by a cluster: fewer stages, and 64 KB for
-constexpr int kPartBytes = 32 * 32 * 4;        // the partial sums of its chunks
-static_assert(2 * kSplitStages * kOperand + 16 * kPartBytes <= 2 * kStages * kOperand, "partial sums");
-constexpr int kSmemBytes = 1024 + kStages * 2 * kOperand + kEpiWarps * kWarpBytes + 512;
+constexpr int kPartBytes = 32 * 32 * 4;        // partial sums of a chunk
+constexpr int kSmemBytes = 1024 + kRing + kEpiWarps * kWarpBytes + 512;
 constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
 
 // Split products: the tensor core truncates as it accumulates, which over a long K costs a few bits of
@@ -343,17 +341,17 @@ __device__ __forceinline__ void tma_store_3d_at(const CUtensorMap* map, uint32_t
                : "memory");
 }
 
-// Unit -> (matrix, tile row, tile column).  The symmetric products enumerate the tiles on and below
-// the diagonal only.
-template <bool SYM>
+// Unit -> (matrix, tile row, tile column).  The symmetric products enumerate the tiles that reach the
+// diagonal or lie below it only: R (tile rows over tile columns) more in every tile row.
+template <bool SYM, int R>
 __device__ __forceinline__ void decode(const GemmParams& p, int u, int& b, int& tm, int& tn) {
   b = u / p.per_batch;
   const int t = u - b * p.per_batch;
   if (SYM) {
-    tm = static_cast<int>((sqrtf(8.f * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
-    while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
-    while (tm * (tm + 1) / 2 > t) --tm;
-    tn = t - tm * (tm + 1) / 2;
+    tm = static_cast<int>((sqrtf(8.f / R * static_cast<float>(t) + 1.f) - 1.f) * 0.5f);
+    while (R * (tm + 1) * (tm + 2) / 2 <= t) ++tm;
+    while (R * tm * (tm + 1) / 2 > t) --tm;
+    tn = t - R * tm * (tm + 1) / 2;
   } else {
     tm = t / p.tiles_n;
     tn = t - tm * p.tiles_n;
@@ -508,19 +506,22 @@ struct Maps {
 
 // KS (CG = 1): the blocks of K are shared by a cluster of `splits` CTAs, which sum their accumulators over
 // distributed shared memory and finish a share of the tile each.
-template <int CG, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
+template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmParams p) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
-  constexpr int BN = BM * CG;  // tile columns (and rows of the pair's tile)
+  constexpr int R = CG * BM / BN;     // a tile is R times as high as wide
+  constexpr int kCols = BN / CG;      // columns of the tile whose operand rows this CTA loads
+  constexpr int kOperandB = kCols * BK * 2;
   constexpr int kTmemCols = 2 * BN;
-  constexpr int kSt = KS ? kSplitStages : kStages;
+  constexpr int kSums = KS ? BN / 32 * 4 * kPartBytes : 0;
+  constexpr int kSt = (kRing - kSums) / (kOperand + kOperandB) > 6 ? 6 : (kRing - kSums) / (kOperand + kOperandB);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + kSt * kOperand;
-  uint8_t* sRed = smem + 2 * kSplitStages * kOperand;  // KS: 16 chunks of partial sums per CTA of the cluster
-  uint8_t* sEpi = smem + 2 * kStages * kOperand;
+  uint8_t* sRed = smem + kSt * (kOperand + kOperandB);  // KS: partial sums of this CTA's share of the tile
+  uint8_t* sEpi = smem + kRing;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + kEpiWarps * kWarpBytes);
   uint64_t* full_bar = bars;
   uint64_t* empty_bar = bars + kSt;
@@ -575,8 +576,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int blocks = p.k_blocks * (SPLIT ? 3 : 1);
   const int lo = KS ? blocks * part / p.splits : 0, hi = KS ? blocks * (part + 1) / p.splits : blocks;
   const int run = SPLIT ? kSplitRun : blocks;  // blocks that one accumulator adds up
-  // A tile on the diagonal of X X^T or A A: both operands are the same rows, loaded once.
-  auto same = [&](int tm, int tn, int i) { return SYM && tm == tn && i < p.k_blocks; };
+  // A tile on the diagonal of X X^T or A A: this CTA's rows of B are among its rows of A, loaded once.
+  auto same = [&](int tm, int tn, int i) { return SYM && tn / R == tm && i < p.k_blocks; };
   if (warp == 0 && lane == 0) {
     // ---------------------------------------------------------- producer
     int stage = 0;
@@ -586,9 +587,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     bool ok = true;
     for (int u = first; u < p.units && ok; u += stride) {
       int b, tm, tn;
-      decode<SYM>(p, u, b, tm, tn);
+      decode<SYM, R>(p, u, b, tm, tn);
       const int row = tm * (CG * BM) + static_cast<int>(crank) * BM;
-      const int col = tn * BN + static_cast<int>(crank) * BM;
+      const int col = tn * BN + static_cast<int>(crank) * kCols;
       for (int i = lo; i < hi; ++i) {
         // high x high, high x low, low x high
         const int which = i / p.k_blocks, k = (i - which * p.k_blocks) * BK;
@@ -601,10 +602,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         uint32_t bar = smem_u32(&full_bar[stage]);
         if constexpr (CG == 2) bar = map_to_cta(bar, 0);
         const bool once = same(tm, tn, i);
-        if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * (once ? 1 : 2) * kOperand);
+        if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * (kOperand + (once ? 0 : kOperandB)));
         armed[stage] = static_cast<int>(phase);
         uint8_t* da = sA + stage * kOperand;
-        uint8_t* db = sB + stage * kOperand;
+        uint8_t* db = sB + stage * kOperandB;
         if (A_MN) {
           load_tile<CG>(ta, bar, da, row, k, b);
           load_tile<CG>(ta, bar, da + kOperand / 2, row + 64, k, b);
@@ -613,8 +614,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         if (once) {
         } else if (B_MN) {
-          load_tile<CG>(tb, bar, db, col, k, b);
-          load_tile<CG>(tb, bar, db + kOperand / 2, col + 64, k, b);
+#pragma unroll
+          for (int c = 0; c < kCols / 64; ++c) load_tile<CG>(tb, bar, db + c * (kOperand / 2), col + c * 64, k, b);
         } else {
           load_tile<CG>(tb, bar, db, k, col, b);
         }
@@ -640,7 +641,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     bool ok = true;
     for (int u = first; u < p.units && ok; u += stride) {
       int b, tm, tn;
-      decode<SYM>(p, u, b, tm, tn);
+      decode<SYM, R>(p, u, b, tm, tn);
       for (int i0 = lo; i0 < hi; i0 += run) {
         if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.status, 422, abort_flag)) {
           ok = false;
@@ -656,7 +657,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
           tc_fence_after();
           const uint64_t a_st = a_base + static_cast<uint32_t>(stage * kOperand >> 4);
-          const uint64_t b_st = (same(tm, tn, i) ? a_base : b_base) + static_cast<uint32_t>(stage * kOperand >> 4);
+          // (64 rows of a stage, in either order, are half an operand on)
+          const uint64_t b_st = same(tm, tn, i) ? a_st + static_cast<uint32_t>((tn % R) * (kOperand / 2) >> 4)
+                                                : b_base + static_cast<uint32_t>(stage * kOperandB >> 4);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
             mma<CG>(d_tmem, a_st + (A_MN ? k * (2048 >> 4) : k * (32 >> 4)), b_st + (B_MN ? k * (2048 >> 4) : k * (32 >> 4)),
@@ -831,11 +834,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     auto wanted = [&](int row0, int n0) { return row0 < p.M && n0 < p.N && (!SYM || n0 <= row0); };
 
     if constexpr (KS) {
-      // The tile's 16 chunks are dealt to the CTAs: chunk t (columns t / 4, rows t % 4) belongs to CTA
+      // The tile's chunks are dealt to the CTAs: chunk t (columns t / 4, rows t % 4) belongs to CTA
       // t / per, warp t % per there.
       int b, tm, tn;
-      decode<SYM>(p, first, b, tm, tn);
-      const int per = 16 / p.splits, mine = part * per + (warp - 2);
+      decode<SYM, R>(p, first, b, tm, tn);
+      const int per = BN / 32 * 4 / p.splits, mine = part * per + (warp - 2);
       const int row0 = tm * BM + (mine & 3) * 32, n0 = tn * BN + (mine >> 2) * 32;
       const bool has = warp - 2 < per && wanted(row0, n0);
       if (kAddend && has) fetch(ctr, b, row0, n0);
@@ -892,7 +895,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     } else {
       for (int u = first; u < p.units && ok; u += stride) {
         int b, tm, tn;
-        decode<SYM>(p, u, b, tm, tn);
+        decode<SYM, R>(p, u, b, tm, tn);
         const int row0 = tm * (CG * BM) + static_cast<int>(crank) * BM + quarter * 32;
         const int col0 = tn * BN + half * kChunks * 32;
         int chunks = 0;  // (those wanted come first)
@@ -961,13 +964,13 @@ bool get_encoder() {
 }
 
 // A stack of fp16 matrices and its tensor maps: operand tiles of 64 columns x 128 rows (K-major) or
-// 64 columns x 64 rows (MN-major), whichever its products take, and epilogue chunks of 32 x 32.
+// 64 columns x 64 rows (K-major for narrow tiles, MN-major), and epilogue chunks of 32 x 32.
 // Columns and rows past the matrix read as zero and are not written.
 struct Stack {
-  CUtensorMap k_major, mn_major, chunk;
-  bool make(void* ptr, int rows, int cols, int count, bool k, bool mn) {
-    return (!k || encode(&k_major, ptr, rows, cols, count, 64, 128)) &&
-           (!mn || encode(&mn_major, ptr, rows, cols, count, 64, 64)) && encode(&chunk, ptr, rows, cols, count, 32, 32);
+  CUtensorMap by_128, by_64, chunk;
+  bool make(void* ptr, int rows, int cols, int count) {
+    return encode(&by_128, ptr, rows, cols, count, 64, 128) && encode(&by_64, ptr, rows, cols, count, 64, 64) &&
+           encode(&chunk, ptr, rows, cols, count, 32, 32);
   }
   static bool encode(CUtensorMap* map, void* ptr, int rows, int cols, int count, cuuint32_t box_cols, cuuint32_t box_rows) {
     const cuuint64_t ld = static_cast<cuuint64_t>(cols + 7) / 8 * 16;
@@ -986,6 +989,13 @@ struct Pair {
   Stack part[2];
 };
 
+int tiles(int n, int t) { return (n + t - 1) / t; }
+// Tiles of height x width that a product computes per matrix: all, or those that reach the diagonal.
+long long tiles_of(bool sym, int rows, int cols, int height, int width) {
+  const long long m = tiles(rows, height), n = tiles(cols, width), r = height / width;
+  return sym ? r * m * (m - 1) / 2 + n : m * n;
+}
+
 int sms() {
   static int n = 0;
   if (n == 0) {
@@ -996,17 +1006,16 @@ int sms() {
   return n;
 }
 
-template <int CG, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
+template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
 cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p, int count,
                            cudaStream_t stream) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
-  constexpr int tile = BM * CG;
-  p.tiles_m = (p.M + tile - 1) / tile;
-  p.tiles_n = (p.N + tile - 1) / tile;
-  p.per_batch = SYM ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+  p.tiles_m = tiles(p.M, BM * CG);
+  p.tiles_n = tiles(p.N, BN);
+  p.per_batch = static_cast<int>(tiles_of(SYM, p.M, p.N, BM * CG, BN));
   p.units = p.per_batch * count;
   p.k_blocks = (p.K + BK - 1) / BK;
-  auto kern = product_kernel<CG, KS, SPLIT, A_MN, B_MN, MODE>;
+  auto kern = product_kernel<CG, BN, KS, SPLIT, A_MN, B_MN, MODE>;
   static int done[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1038,36 +1047,37 @@ cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pa
   }
   Maps maps;
   for (int i = 0; i < 2; ++i) {
-    maps.a[i] = A_MN ? a.part[i].mn_major : a.part[i].k_major;
-    maps.b[i] = B_MN ? b.part[i].mn_major : b.part[i].k_major;
+    maps.a[i] = A_MN ? a.part[i].by_64 : a.part[i].by_128;
+    maps.b[i] = B_MN || BN / CG == 64 ? b.part[i].by_64 : b.part[i].by_128;
     maps.c[i] = c.part[i].chunk;
     maps.d[i] = d.part[i].chunk;
   }
   return cudaLaunchKernelEx(&cfg, kern, maps, p);
 }
 
-// How a product is cut.  `tile`: 0 choose, 1: 128 x 128 tiles, 2: 256 x 256 tiles on SM pairs.
+// How a product is cut.  `tile`: 0 choose, 1: 128 x 128 tiles, 2: 256 x 256 tiles on SM pairs
+// (not split products), 3: 128 x 64.
 template <bool A_MN, bool B_MN, int MODE>
 cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p,
                     int count, cudaStream_t s) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
-  auto units = [&](int t) {
-    const long long m = (p.M + t - 1) / t, n = (p.N + t - 1) / t;
-    return (SYM ? m * (m + 1) / 2 : m * n) * count;
-  };
-  // Few tiles: K is shared by as many CTAs as fit the SMs together and keep four blocks each.
-  const int blocks = (p.K + BK - 1) / BK * (split ? 3 : 1);
+  auto units = [&](int height, int width) { return tiles_of(SYM, p.M, p.N, height, width) * count; };
   p.splits = 1;
-  if (tile == 0)
-    while (p.splits < 8 && units(BM) * 2 * p.splits <= sms() && blocks >= 8 * p.splits) p.splits *= 2;
-  if (p.splits > 1)
-    return split ? launch_product<1, true, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)
-                 : launch_product<1, true, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
-  if (split) return launch_product<1, false, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  if (tile == 3 || (tile == 0 && units(BM, 64) <= sms())) {
+    // Few tiles: narrow ones, and K shared by as many CTAs as fit the SMs together and keep two blocks each.
+    const int blocks = tiles(p.K, BK) * (split ? 3 : 1);
+    while (p.splits < 8 && units(BM, 64) * 2 * p.splits <= sms() && blocks >= 4 * p.splits) p.splits *= 2;
+    if (p.splits > 1)
+      return split ? launch_product<1, 64, true, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)
+                   : launch_product<1, 64, true, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+    return split ? launch_product<1, 64, false, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)
+                 : launch_product<1, 64, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  }
+  if (split) return launch_product<1, 128, false, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
   // Pairs of SMs where their larger tiles still occupy half of the SMs.
-  if (tile == 2 || (tile == 0 && units(2 * BM) >= sms() / 4))
-    return launch_product<2, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
-  return launch_product<1, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  if (tile == 2 || (tile == 0 && units(2 * BM, 2 * BM) >= sms() / 4))
+    return launch_product<2, 256, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
+  return launch_product<1, 128, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
 }
 
 struct Layout {  // byte offsets in the workspace (each 256-byte aligned)
@@ -1138,10 +1148,10 @@ extern "C" int md_muon(const MdMuonParams* prm, cudaStream_t stream) {
   Pair x[2], a{}, f{};
   bool ok = true;
   for (int i = 0; i < 2; ++i)
-    for (int w = 0; w < 2; ++w) ok = ok && x[i].part[w].make(ws + l.x[i][w], p.rows, p.cols, p.count, true, true);
+    for (int w = 0; w < 2; ++w) ok = ok && x[i].part[w].make(ws + l.x[i][w], p.rows, p.cols, p.count);
   for (int w = 0; w <= static_cast<int>(split); ++w)
-    ok = ok && a.part[w].make(ws + l.a[w], small, small, p.count, true, false) &&
-         f.part[w].make(ws + l.f[w], small, small, p.count, true, false);
+    ok = ok && a.part[w].make(ws + l.a[w], small, small, p.count) &&
+         f.part[w].make(ws + l.f[w], small, small, p.count);
   if (!ok) return -8;
 
   cudaError_t e = p.step           ? prepare<float, true>(p, l, static_cast<int>(chunks), stream)

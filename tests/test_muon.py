@@ -73,12 +73,13 @@ def test_orthogonalize(device, dtype, shape):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tile", [0, 1, 2])
+@pytest.mark.parametrize("tile", [0, 1, 2, 3])
 @pytest.mark.parametrize("shape", [(3, 70, 40), (2, 256, 256), (2, 300, 700), (3, 700, 300), (1, 1100, 1030),
                                    (70, 40, 24)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_tiles_and_batches(tile, shape, dtype):
-    """Both tile sizes, and the choice (K shared by a cluster where tiles are few), at sizes that end inside a tile, several tiles per SM, more matrices than a call takes."""
+    """Every tile size, and the choice, at sizes that end inside a tile, with K shared by a cluster, several
+    tiles per SM, more matrices than a call takes."""
     u = _matrix(*shape, seed=1, decay=dtype == torch.bfloat16).to("cuda", dtype)
     x = M._orthogonalize_cuda(u, 5, M.COEFFICIENTS, 1e-7, tile=tile)
     nat.check_status()

@@ -219,11 +219,6 @@ constexpr int kPartBytes = 32 * 32 * 4;        // partial sums of a chunk
 constexpr int kSmemBytes = 1024 + kRing + kEpiWarps * kWarpBytes + 512;
 constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
 
-// Split products: the tensor core truncates as it accumulates, which over a long K costs a few bits of
-// the 22.  After this many blocks of K the accumulator is added to fp32 registers and starts again
-// (measured error of a 1100 x 1030 answer: 1.3e-5 in one accumulation).
-constexpr int kSplitRun = 2;
-
 enum Mode : int { kGram = 0, kPoly = 1, kNext = 2, kLast = 3 };
 
 struct GemmParams {
@@ -504,6 +499,10 @@ struct Maps {
   CUtensorMap a[2], b[2], c[2], d[2];  // high and low parts: operands, addend, result
 };
 
+// SPLIT: a stage holds both parts of both operands, loaded once for the three products of a block of K:
+// low x high and high x low first, then high x high.  The tensor core truncates as it accumulates, which
+// over a long K would cost a few bits of the 22, so every block's sum is added up in fp32 registers
+// (error of a 1100 x 1030 answer: 1.3e-5 in one accumulation over K, MEASURED so).
 // KS (CG = 1): the blocks of K are shared by a cluster of `splits` CTAs, which sum their accumulators over
 // distributed shared memory and finish a share of the tile each.
 template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
@@ -514,13 +513,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   constexpr int kCols = BN / CG;      // columns of the tile whose operand rows this CTA loads
   constexpr int kOperandB = kCols * BK * 2;
   constexpr int kTmemCols = 2 * BN;
+  constexpr int kParts = SPLIT ? 2 : 1;
+  constexpr int kStage = kParts * (kOperand + kOperandB);
   constexpr int kSums = KS ? BN / 32 * 4 * kPartBytes : 0;
-  constexpr int kSt = (kRing - kSums) / (kOperand + kOperandB) > 6 ? 6 : (kRing - kSums) / (kOperand + kOperandB);
+  constexpr int kSt = (kRing - kSums) / kStage > 6 ? 6 : (kRing - kSums) / kStage;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = smem + kSt * kOperand;
-  uint8_t* sRed = smem + kSt * (kOperand + kOperandB);  // KS: partial sums of this CTA's share of the tile
+  uint8_t* sB = smem + kSt * kParts * kOperand;
+  uint8_t* sRed = smem + kSt * kStage;  // KS: partial sums of this CTA's share of the tile
   uint8_t* sEpi = smem + kRing;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sEpi + kEpiWarps * kWarpBytes);
   uint64_t* full_bar = bars;
@@ -573,11 +574,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   pdl_trigger();
   pdl_wait();
 
-  const int blocks = p.k_blocks * (SPLIT ? 3 : 1);
-  const int lo = KS ? blocks * part / p.splits : 0, hi = KS ? blocks * (part + 1) / p.splits : blocks;
-  const int run = SPLIT ? kSplitRun : blocks;  // blocks that one accumulator adds up
+  const int lo = KS ? p.k_blocks * part / p.splits : 0, hi = KS ? p.k_blocks * (part + 1) / p.splits : p.k_blocks;
+  const int run = SPLIT ? 1 : p.k_blocks;  // blocks that one accumulator adds up
   // A tile on the diagonal of X X^T or A A: this CTA's rows of B are among its rows of A, loaded once.
-  auto same = [&](int tm, int tn, int i) { return SYM && tn / R == tm && i < p.k_blocks; };
+  auto same = [&](int tm, int tn) { return SYM && tn / R == tm; };
   if (warp == 0 && lane == 0) {
     // ---------------------------------------------------------- producer
     int stage = 0;
@@ -591,33 +591,34 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int row = tm * (CG * BM) + static_cast<int>(crank) * BM;
       const int col = tn * BN + static_cast<int>(crank) * kCols;
       for (int i = lo; i < hi; ++i) {
-        // high x high, high x low, low x high
-        const int which = i / p.k_blocks, k = (i - which * p.k_blocks) * BK;
-        const CUtensorMap* ta = &maps.a[which == 2];
-        const CUtensorMap* tb = &maps.b[which == 1];
+        const int k = i * BK;
         if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, 420, abort_flag)) {
           ok = false;
           break;
         }
         uint32_t bar = smem_u32(&full_bar[stage]);
         if constexpr (CG == 2) bar = map_to_cta(bar, 0);
-        const bool once = same(tm, tn, i);
-        if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * (kOperand + (once ? 0 : kOperandB)));
+        const bool once = same(tm, tn);
+        if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * kParts * (kOperand + (once ? 0 : kOperandB)));
         armed[stage] = static_cast<int>(phase);
-        uint8_t* da = sA + stage * kOperand;
-        uint8_t* db = sB + stage * kOperandB;
-        if (A_MN) {
-          load_tile<CG>(ta, bar, da, row, k, b);
-          load_tile<CG>(ta, bar, da + kOperand / 2, row + 64, k, b);
-        } else {
-          load_tile<CG>(ta, bar, da, k, row, b);
-        }
-        if (once) {
-        } else if (B_MN) {
 #pragma unroll
-          for (int c = 0; c < kCols / 64; ++c) load_tile<CG>(tb, bar, db + c * (kOperand / 2), col + c * 64, k, b);
-        } else {
-          load_tile<CG>(tb, bar, db, k, col, b);
+        for (int w = 0; w < kParts; ++w) {
+          uint8_t* da = sA + (stage * kParts + w) * kOperand;
+          uint8_t* db = sB + (stage * kParts + w) * kOperandB;
+          if (A_MN) {
+            load_tile<CG>(&maps.a[w], bar, da, row, k, b);
+            load_tile<CG>(&maps.a[w], bar, da + kOperand / 2, row + 64, k, b);
+          } else {
+            load_tile<CG>(&maps.a[w], bar, da, k, row, b);
+          }
+          if (once) continue;
+          if (B_MN) {
+#pragma unroll
+            for (int c = 0; c < kCols / 64; ++c)
+              load_tile<CG>(&maps.b[w], bar, db + c * (kOperand / 2), col + c * 64, k, b);
+          } else {
+            load_tile<CG>(&maps.b[w], bar, db, k, col, b);
+          }
         }
         if (++stage == kSt) {
           stage = 0;
@@ -656,14 +657,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint64_t a_st = a_base + static_cast<uint32_t>(stage * kOperand >> 4);
+          const uint64_t a_st = a_base + static_cast<uint32_t>(stage * kParts * kOperand >> 4);
           // (64 rows of a stage, in either order, are half an operand on)
-          const uint64_t b_st = same(tm, tn, i) ? a_st + static_cast<uint32_t>((tn % R) * (kOperand / 2) >> 4)
-                                                : b_base + static_cast<uint32_t>(stage * kOperandB >> 4);
+          const bool once = same(tm, tn);
+          const uint64_t b_st = once ? a_st + static_cast<uint32_t>((tn % R) * (kOperand / 2) >> 4)
+                                     : b_base + static_cast<uint32_t>(stage * kParts * kOperandB >> 4);
+          const uint32_t b_low = static_cast<uint32_t>((once ? kOperand : kOperandB) >> 4);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            mma<CG>(d_tmem, a_st + (A_MN ? k * (2048 >> 4) : k * (32 >> 4)), b_st + (B_MN ? k * (2048 >> 4) : k * (32 >> 4)),
-                    idesc, (i > i0 || k > 0) ? 1u : 0u);
+          for (int t = SPLIT ? 0 : 2; t < 3; ++t) {  // low x high, high x low, high x high
+            const uint64_t at = a_st + (t == 0 ? static_cast<uint32_t>(kOperand >> 4) : 0u);
+            const uint64_t bt = b_st + (t == 1 ? b_low : 0u);
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k)
+              mma<CG>(d_tmem, at + (A_MN ? k * (2048 >> 4) : k * (32 >> 4)), bt + (B_MN ? k * (2048 >> 4) : k * (32 >> 4)),
+                      idesc, (i > i0 || k > 0 || (SPLIT && t > 0)) ? 1u : 0u);
+          }
           commit_all<CG>(&empty_bar[stage]);
           if (++stage == kSt) {
             stage = 0;
@@ -1064,8 +1072,9 @@ cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pa
   auto units = [&](int height, int width) { return tiles_of(SYM, p.M, p.N, height, width) * count; };
   p.splits = 1;
   if (tile == 3 || (tile == 0 && units(BM, 64) <= sms())) {
-    // Few tiles: narrow ones, and K shared by as many CTAs as fit the SMs together and keep two blocks each.
-    const int blocks = tiles(p.K, BK) * (split ? 3 : 1);
+    // Few tiles: narrow ones, and K shared by as many CTAs as fit the SMs together and keep two blocks
+    // (of split products one) each.
+    const int blocks = tiles(p.K, BK) * (split ? 2 : 1);
     while (p.splits < 8 && units(BM, 64) * 2 * p.splits <= sms() && blocks >= 4 * p.splits) p.splits *= 2;
     if (p.splits > 1)
       return split ? launch_product<1, 64, true, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)

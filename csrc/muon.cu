@@ -262,22 +262,34 @@ __device__ __forceinline__ void cluster_join() {
 }
 
 // Tile load whose bytes are counted on `bar`: this CTA's barrier, or with CG = 2 the pair
-// leader's (cluster address).
+// leader's (cluster address).  By a whole warp, one elected lane issues: addresses and
+// coordinates stay in uniform registers.
 template <int CG>
-__device__ __forceinline__ void load_tile(const CUtensorMap* map, uint32_t bar, void* dst, int x, int y, int z) {
+__device__ __forceinline__ void load_tile(const CUtensorMap* map, uint32_t bar, const uint8_t* dst, int x, int y, int z) {
   if constexpr (CG == 2) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n\t}\n" ::"r"(smem_u32(dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
   } else {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n\t}\n" ::"r"(smem_u32(dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
   }
+}
+__device__ __forceinline__ void expect_elect(uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t.reg .b32 r;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(smem_u32(bar)), "r"(bytes)
+      : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -578,8 +590,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int run = SPLIT ? 1 : p.k_blocks;  // blocks that one accumulator adds up
   // A tile on the diagonal of X X^T or A A: this CTA's rows of B are among its rows of A, loaded once.
   auto same = [&](int tm, int tn) { return SYM && tn / R == tm; };
-  if (warp == 0 && lane == 0) {
-    // ---------------------------------------------------------- producer
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer (whole warp, elected lane issues)
     int stage = 0;
     uint32_t phase = 0;
     int armed[kSt];
@@ -592,14 +604,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int col = tn * BN + static_cast<int>(crank) * kCols;
       for (int i = lo; i < hi; ++i) {
         const int k = i * BK;
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, 420, abort_flag)) {
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, 420, abort_flag))) {
           ok = false;
           break;
         }
         uint32_t bar = smem_u32(&full_bar[stage]);
         if constexpr (CG == 2) bar = map_to_cta(bar, 0);
         const bool once = same(tm, tn);
-        if (leader) mbar_arrive_expect_tx(&full_bar[stage], CG * kParts * (kOperand + (once ? 0 : kOperandB)));
+        if (leader) expect_elect(&full_bar[stage], CG * kParts * (kOperand + (once ? 0 : kOperandB)));
         armed[stage] = static_cast<int>(phase);
 #pragma unroll
         for (int w = 0; w < kParts; ++w) {

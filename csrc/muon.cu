@@ -545,7 +545,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * kSt + 6);
   uint64_t* c_bar = bars + 2 * kSt + 7;  // two per epilogue warp
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (Through a shuffle: the compiler then knows that a warp's role is the same for all its lanes, and
+  // keeps the issuing loops' addresses and descriptors in uniform registers.)
+  const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t crank = CG == 2 ? cluster_ctarank() : 0u;
   const int part = KS ? static_cast<int>(cluster_ctarank()) : 0;
   const bool leader = crank == 0;

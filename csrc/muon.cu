@@ -43,6 +43,8 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <type_traits>
+
 #include "md_sm100.cuh"
 
 constexpr int kMuonBatch = 64;  // matrices per call
@@ -231,9 +233,13 @@ struct GemmParams {
   const float* lr;
   const float* skip;
   Status* status;
+};
+struct LastParams : GemmParams {  // (1 KB of pointers, which the other launches need not carry)
   void* out[kMuonBatch];
   __nv_bfloat16* shadow[kMuonBatch];
 };
+template <int MODE>
+using Params = std::conditional_t<MODE == kLast, LastParams, GemmParams>;
 
 // kind::f16 with f16 operands, fp32 accumulators.
 constexpr uint32_t idesc_f16(int M, int N, bool a_mn, bool b_mn) {
@@ -291,18 +297,37 @@ __device__ __forceinline__ void expect_elect(uint64_t* bar, uint32_t bytes) {
       "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(smem_u32(bar)), "r"(bytes)
       : "memory");
 }
-template <int CG>
-__device__ __forceinline__ void mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The four MMAs of a block of K (their descriptors are a step of 16 of K apart), by one elected lane.
+template <int CG, int kStepA, int kStepB>
+__device__ __forceinline__ void mma_block(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  static_assert(BK == 64);
   if constexpr (CG == 2) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+        "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "add.s64 a1, %1, %5;\n\tadd.s64 a2, a1, %5;\n\tadd.s64 a3, a2, %5;\n\t"
+        "add.s64 b1, %2, %6;\n\tadd.s64 b2, b1, %6;\n\tadd.s64 b3, b2, %6;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
         "elect.sync r|e, 0xffffffff;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a1, b1, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a2, b2, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::2.kind::f16 [%0], a3, b3, %3, t;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(kStepA), "n"(kStepB)
         : "memory");
   } else {
-    umma_bf16_ss_elect(tmem_d, adesc, bdesc, idesc, accumulate);  // (the element type is in idesc)
+    asm volatile(
+        "{\n\t.reg .pred p, t, e;\n\t.reg .b32 r;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "add.s64 a1, %1, %5;\n\tadd.s64 a2, a1, %5;\n\tadd.s64 a3, a2, %5;\n\t"
+        "add.s64 b1, %2, %6;\n\tadd.s64 b2, b1, %6;\n\tadd.s64 b3, b2, %6;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %4, %4;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(kStepA), "n"(kStepB)
+        : "memory");
   }
 }
 // Arrive on `bar` in every CTA of the pair once the MMAs issued so far are complete.
@@ -427,7 +452,7 @@ struct Out {
   float rate, decay;
   bool idle, wide;  // nothing to write; rows and addresses allow whole pieces
 };
-__device__ __forceinline__ void load_old(const GemmParams& p, const Out& o, int b, int row0, int n0, int lane, float4 (&old)[8]) {
+__device__ __forceinline__ void load_old(const LastParams& p, const Out& o, int b, int row0, int n0, int lane, float4 (&old)[8]) {
   const int col = n0 + (lane & 7) * 4;
   if (!p.step || !o.wide || o.idle || col >= p.N) return;
   const float* w = static_cast<const float*>(p.out[b]) + static_cast<long long>(row0 + (lane >> 3)) * p.N + col;
@@ -435,7 +460,7 @@ __device__ __forceinline__ void load_old(const GemmParams& p, const Out& o, int 
   for (int i = 0; i < 8; ++i)
     if (row0 + 4 * i + (lane >> 3) < p.M) old[i] = *reinterpret_cast<const float4*>(w + 4ll * i * p.N);
 }
-__device__ __forceinline__ void write_out(const GemmParams& p, const Out& o, uint32_t staged, int b, int row0, int n0,
+__device__ __forceinline__ void write_out(const LastParams& p, const Out& o, uint32_t staged, int b, int row0, int n0,
                                           int lane, const float4 (&old)[8]) {
   if (o.idle) return;
   const int col = n0 + (lane & 7) * 4;
@@ -519,7 +544,7 @@ struct Maps {
 // distributed shared memory and finish a share of the tile each.
 template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ GemmParams p) {
+    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params<MODE> p) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
   constexpr int R = CG * BM / BN;     // a tile is R times as high as wide
   constexpr int kCols = BN / CG;      // columns of the tile whose operand rows this CTA loads
@@ -681,10 +706,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           for (int t = SPLIT ? 0 : 2; t < 3; ++t) {  // low x high, high x low, high x high
             const uint64_t at = a_st + (t == 0 ? static_cast<uint32_t>(kOperand >> 4) : 0u);
             const uint64_t bt = b_st + (t == 1 ? b_low : 0u);
-#pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              mma<CG>(d_tmem, at + (A_MN ? k * (2048 >> 4) : k * (32 >> 4)), bt + (B_MN ? k * (2048 >> 4) : k * (32 >> 4)),
-                      idesc, (i > i0 || k > 0 || (SPLIT && t > 0)) ? 1u : 0u);
+            mma_block<CG, A_MN ? 128 : 2, B_MN ? 128 : 2>(d_tmem, at, bt, idesc,
+                                                          (i > i0 || (SPLIT && t > 0)) ? 1u : 0u);
           }
           commit_all<CG>(&empty_bar[stage]);
           if (++stage == kSt) {
@@ -761,14 +784,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     Out out;
     float4 old[8];
     auto prepare_out = [&](int b, int row0, int n0) {
-      const float lr = p.lr != nullptr ? *p.lr : 1.f;
-      out.rate = p.step ? -p.rate * lr * (1.f / kScale) : 1.f / kScale;
-      out.decay = p.lr != nullptr ? 1.f - lr * p.decay : p.decay;
-      out.idle = p.step && p.skip != nullptr && *p.skip != 0.f;
-      const unsigned long long piece = p.dtype == 2 ? 15u : 7u;
-      out.wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out[b]) & piece) == 0 &&
-                 (reinterpret_cast<uintptr_t>(p.shadow[b]) & 7u) == 0;
-      load_old(p, out, b, row0, n0, lane, old);
+      if constexpr (MODE == kLast) {
+        const float lr = p.lr != nullptr ? *p.lr : 1.f;
+        out.rate = p.step ? -p.rate * lr * (1.f / kScale) : 1.f / kScale;
+        out.decay = p.lr != nullptr ? 1.f - lr * p.decay : p.decay;
+        out.idle = p.step && p.skip != nullptr && *p.skip != 0.f;
+        const unsigned long long piece = p.dtype == 2 ? 15u : 7u;
+        out.wide = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out[b]) & piece) == 0 &&
+                   (reinterpret_cast<uintptr_t>(p.shadow[b]) & 7u) == 0;
+        load_old(p, out, b, row0, n0, lane, old);
+      }
     };
     auto load_acc = [&](int c, float (&v)[32]) {  // this warp's chunk c of the current accumulator
       uint32_t r[32];
@@ -1029,7 +1054,7 @@ int sms() {
 }
 
 template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
-cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p, int count,
+cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pair& d, LastParams& p, int count,
                            cudaStream_t stream) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
   p.tiles_m = tiles(p.M, BM * CG);
@@ -1074,13 +1099,13 @@ cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pa
     maps.c[i] = c.part[i].chunk;
     maps.d[i] = d.part[i].chunk;
   }
-  return cudaLaunchKernelEx(&cfg, kern, maps, p);
+  return cudaLaunchKernelEx(&cfg, kern, maps, static_cast<const Params<MODE>&>(p));
 }
 
 // How a product is cut.  `tile`: 0 choose, 1: 128 x 128 tiles, 2: 256 x 256 tiles on SM pairs
 // (not split products), 3: 128 x 64.
 template <bool A_MN, bool B_MN, int MODE>
-cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pair& c, const Pair& d, GemmParams& p,
+cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pair& c, const Pair& d, LastParams& p,
                     int count, cudaStream_t s) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
   auto units = [&](int height, int width) { return tiles_of(SYM, p.M, p.N, height, width) * count; };
@@ -1183,7 +1208,7 @@ extern "C" int md_muon(const MdMuonParams* prm, cudaStream_t stream) {
                                    : prepare<float, false>(p, l, static_cast<int>(chunks), stream);
   if (e != cudaSuccess) return static_cast<int>(e);
 
-  GemmParams g{};
+  LastParams g{};
   g.status = p.status;
   g.dtype = p.dtype, g.step = p.step;
   g.decay = p.decay, g.rate = p.rate, g.lr = p.lr, g.skip = p.skip;

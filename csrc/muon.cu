@@ -43,6 +43,7 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <iterator>
 #include <type_traits>
 
 #include "md_sm100.cuh"
@@ -67,7 +68,7 @@ struct MdMuonParams {
   const float* skip;        // null, or device flag: nonzero leaves everything as it is
   void* workspace;
   long long workspace_bytes;
-  int tile;                 // 0 choose, 1: 128 x 128 tiles, 2: 256 x 256 tiles on SM pairs
+  int tile;                 // 0 choose, 1: 128 x 128 tiles, 2: 256 x 256 tiles on SM pairs, 3: 128 x 64
   md::Status* status;
   const void* src[kMuonBatch];
   float* m[kMuonBatch];
@@ -104,9 +105,20 @@ __device__ __forceinline__ float block_sum(float v) {
   return t;
 }
 
+// What the first two kernels need (an argument's bytes count in a launch of a few us).
+template <bool STEP>
+struct Source {
+  int rows, cols, nesterov;
+  float momentum, eps;
+  const float *inv_scale, *skip;
+  const void* src[kMuonBatch];
+  float* m[STEP ? kMuonBatch : 1];
+};
+
 // Momentum (step form) and the chunk's share of |U|^2.  grid (chunks, count).
 template <typename T, bool STEP>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ MdMuonParams p, float* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ Source<STEP> p,
+                                                        float* __restrict__ partial) {
   pdl_trigger();
   pdl_wait();
   const int which = blockIdx.y;
@@ -114,7 +126,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ 
   const long long lo = static_cast<long long>(blockIdx.x) * kChunk;
   const long long hi = lo + kChunk < n ? lo + kChunk : n;
   const T* g = static_cast<const T*>(p.src[which]);
-  float* m = p.m[which];
+  float* m = STEP ? p.m[which] : nullptr;
   if (STEP && p.skip != nullptr && *p.skip != 0.f) return;
   const float gs = STEP && p.inv_scale != nullptr ? *p.inv_scale : 1.f;
   float sum = 0.f;
@@ -155,7 +167,7 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
 
 // X = U kScale / (|U| + eps) as high and low fp16 of row stride ldx.  grid (chunks, count).
 template <typename T, bool STEP>
-__global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant__ MdMuonParams p,
+__global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant__ Source<STEP> p,
                                                            const float* __restrict__ partial, __half* __restrict__ xh,
                                                            __half* __restrict__ xl, int ldx) {
   pdl_trigger();
@@ -171,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
   const long long lo = static_cast<long long>(blockIdx.x) * kChunk;
   const long long hi = lo + kChunk < n ? lo + kChunk : n;
   const T* g = static_cast<const T*>(p.src[which]);
-  const float* m = p.m[which];
+  const float* m = STEP ? p.m[which] : nullptr;
   const float gs = STEP && p.inv_scale != nullptr ? *p.inv_scale : 1.f;
   // Position of the chunk's first element; inside the chunk 32-bit division is enough.
   const long long row_lo = lo / p.cols;
@@ -532,8 +544,17 @@ __device__ __forceinline__ void get_staged(uint32_t staged, int lane, float (&v)
                  : "memory");
 }
 
-struct Maps {
-  CUtensorMap a[2], b[2], c[2], d[2];  // high and low parts: operands, addend, result
+// The parts that a product reads and writes: X is a pair throughout, A and B with split products only.
+template <bool SPLIT, int MODE>
+struct Parts {
+  static constexpr bool kAddend = MODE != kGram;
+  static constexpr bool kAddLow = SPLIT || MODE == kNext || MODE == kLast;  // the addend is a pair
+  static constexpr bool kLow = SPLIT || MODE == kNext;  // the result is a pair
+};
+template <bool SPLIT, int MODE>
+struct Maps {  // high and low parts: operands, addend, result
+  using P = Parts<SPLIT, MODE>;
+  CUtensorMap a[SPLIT ? 2 : 1], b[SPLIT ? 2 : 1], d[P::kLow ? 2 : 1], c[P::kAddend && P::kAddLow ? 2 : 1];
 };
 
 // SPLIT: a stage holds both parts of both operands, loaded once for the three products of a block of K:
@@ -544,7 +565,7 @@ struct Maps {
 // distributed shared memory and finish a share of the tile each.
 template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params<MODE> p) {
+    product_kernel(const __grid_constant__ Maps<SPLIT, MODE> maps, const __grid_constant__ Params<MODE> p) {
   constexpr bool SYM = MODE == kGram || MODE == kPoly;
   constexpr int R = CG * BM / BN;     // a tile is R times as high as wide
   constexpr int kCols = BN / CG;      // columns of the tile whose operand rows this CTA loads
@@ -754,9 +775,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     // Staging: slot = the addend's chunk (high, low) on arrival, the result's on departure.  Two slots,
     // so that the next addend arrives under this chunk's arithmetic; one where a result with its
     // mirror image needs both.
-    constexpr bool kAddend = MODE != kGram;
-    constexpr bool kAddLow = SPLIT || MODE == kNext || MODE == kLast;  // X is always a pair, A with split products
-    constexpr bool kLow = SPLIT || MODE == kNext;                      // the result is a pair
+    constexpr bool kAddend = Parts<SPLIT, MODE>::kAddend, kAddLow = Parts<SPLIT, MODE>::kAddLow,
+                   kLow = Parts<SPLIT, MODE>::kLow;
     constexpr int kSlots = SPLIT && SYM ? 1 : 2;
     const uint32_t base = smem_u32(sEpi) + (warp - 2) * kWarpBytes;
     uint64_t* cb = c_bar + (warp - 2) * 2;
@@ -777,7 +797,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const uint32_t dst = base + (i % kSlots) * (kWarpBytes / 2);
         mbar_arrive_expect_tx(bar, kAddLow ? 2 * kChunkBytes : kChunkBytes);
         tma_load_3d_at(&maps.c[0], bar, dst, n0, row0, b);
-        if (kAddLow) tma_load_3d_at(&maps.c[1], bar, dst + kChunkBytes, n0, row0, b);
+        if constexpr (kAddLow) tma_load_3d_at(&maps.c[1], bar, dst + kChunkBytes, n0, row0, b);
       }
     };
     bool ok = true;
@@ -866,10 +886,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         __syncwarp();
         if (lane == 0) {
           tma_store_3d_at(&maps.d[0], slot, n0, row0, b);
-          if (kLow) tma_store_3d_at(&maps.d[1], slot + kChunkBytes, n0, row0, b);
+          if constexpr (kLow) tma_store_3d_at(&maps.d[1], slot + kChunkBytes, n0, row0, b);
           if (SYM && mirrored) {
             tma_store_3d_at(&maps.d[0], slot + kMirror, row0, n0, b);
-            if (kLow) tma_store_3d_at(&maps.d[1], slot + kMirror + kChunkBytes, row0, n0, b);
+            if constexpr (kLow) tma_store_3d_at(&maps.d[1], slot + kMirror + kChunkBytes, row0, n0, b);
           }
           bulk_commit_group();
         }
@@ -1092,13 +1112,13 @@ cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pa
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  Maps maps;
-  for (int i = 0; i < 2; ++i) {
+  Maps<SPLIT, MODE> maps;
+  for (int i = 0; i < static_cast<int>(std::size(maps.a)); ++i) {
     maps.a[i] = A_MN ? a.part[i].by_64 : a.part[i].by_128;
     maps.b[i] = B_MN || BN / CG == 64 ? b.part[i].by_64 : b.part[i].by_128;
-    maps.c[i] = c.part[i].chunk;
-    maps.d[i] = d.part[i].chunk;
   }
+  for (int i = 0; i < static_cast<int>(std::size(maps.c)); ++i) maps.c[i] = c.part[i].chunk;
+  for (int i = 0; i < static_cast<int>(std::size(maps.d)); ++i) maps.d[i] = d.part[i].chunk;
   return cudaLaunchKernelEx(&cfg, kern, maps, static_cast<const Params<MODE>&>(p));
 }
 
@@ -1158,10 +1178,15 @@ template <typename T, bool STEP>
 cudaError_t prepare(const MdMuonParams& p, const Layout& l, int chunks, cudaStream_t s) {
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
   float* partial = reinterpret_cast<float*>(ws + l.partial);
+  Source<STEP> from{p.rows, p.cols, p.nesterov, p.momentum, p.eps, p.inv_scale, p.skip};
+  for (int i = 0; i < p.count; ++i) {
+    from.src[i] = p.src[i];
+    if (STEP) from.m[i] = p.m[i];
+  }
   const dim3 grid(chunks, p.count), block(kThreads);
-  cudaError_t e = launch_pdl(norm_kernel<T, STEP>, grid, block, 0, s, p, partial);
+  cudaError_t e = launch_pdl(norm_kernel<T, STEP>, grid, block, 0, s, from, partial);
   if (e != cudaSuccess) return e;
-  return launch_pdl(convert_kernel<T, STEP>, grid, block, 0, s, p, static_cast<const float*>(partial),
+  return launch_pdl(convert_kernel<T, STEP>, grid, block, 0, s, from, static_cast<const float*>(partial),
                     reinterpret_cast<__half*>(ws + l.x[0][0]), reinterpret_cast<__half*>(ws + l.x[0][1]),
                     (p.cols + 7) / 8 * 8);
 }

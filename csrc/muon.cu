@@ -28,18 +28,19 @@
 // One persistent warp-specialised kernel does every product: TMA loads, one
 // tcgen05.mma issuer, accumulators double-buffered in TMEM so that a tile's
 // epilogue runs under the next one's products.  A tile is 256 x 256 on a pair
-// of SMs (cta_group::2), 128 x 128 on one or, where that leaves SMs idle, 128 x 64;
-// where SMs are idle all the same, a cluster shares the K of each tile and adds
-// the parts up over distributed shared memory.
+// of SMs (cta_group::2) or 128 x 128 on one, by the longest SM's work, or, where
+// that leaves SMs idle, 128 x 64; where SMs are idle all the same, a cluster
+// shares the K of each tile and adds the parts up over distributed shared memory.
 //
 // Measured (B200; cuBLAS bf16 1634 TFLOP/s in bursts, 1395 sustained under the
 // power cap), useful operations, symmetric ones counted once: 4096 x 4096, five
-// steps, 1.16 ms = 1190 TFLOP/s in bursts, 1.39 ms = 990 sustained (tensor pipe
-// active 69 to 78 % of the time; the rest is the last wave of 256 tiles on 74
-// pairs).  12 x 2304 x 768 with momentum and weights 490 us = 555 TFLOP/s: K is 768,
-// so a tile brings 512 KB of addend and result to 768 KB of operands (measured
-// without them: 420 us).  768 x 768 128 us: 17 launches of 7.5 us, each a chain of
-// launch, first load, 12 blocks of K and epilogue, on 21 to 72 of the SMs.
+// steps, 1.09 ms = 1260 TFLOP/s in bursts, 1.33 ms = 1030 sustained (tensor pipe
+// active 76 to 82 % of the time; the rest is the last wave of 256 tiles on 74
+// pairs).  12 x 2304 x 768 with momentum and weights 465 us = 585 TFLOP/s: K is 768,
+// so a tile brings 512 KB of addend and result to 768 KB of operands (tensor pipe
+// 59 % active in X^T X, 40 % in the update).  768 x 768 89 us: 17 launches of 5.3 us,
+// each a chain of launch, first load, 12 blocks of K, of 410 cycles each at the rate
+// at which an SM takes operands from L2, and epilogue, on 42 to 72 of the SMs.
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
@@ -560,7 +561,8 @@ struct Maps {  // high and low parts: operands, addend, result
 // SPLIT: a stage holds both parts of both operands, loaded once for the three products of a block of K:
 // low x high and high x low first, then high x high.  The tensor core truncates as it accumulates, which
 // over a long K would cost a few bits of the 22, so every block's sum is added up in fp32 registers
-// (error of a 1100 x 1030 answer: 1.3e-5 in one accumulation over K, MEASURED so).
+// (errors after five steps: 1.0e-6 at 1000 x 3000, 2.4e-6 at 600 x 5000, as fp32's own products; 1.3e-5
+// at 1100 x 1030 when each product was one accumulation over K).
 // KS (CG = 1): the blocks of K are shared by a cluster of `splits` CTAs, which sum their accumulators over
 // distributed shared memory and finish a share of the tile each.
 template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
@@ -1131,10 +1133,12 @@ cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pa
   auto units = [&](int height, int width) { return tiles_of(SYM, p.M, p.N, height, width) * count; };
   p.splits = 1;
   if (tile == 3 || (tile == 0 && units(BM, 64) <= sms())) {
-    // Few tiles: narrow ones, and K shared by as many CTAs as fit the SMs together and keep two blocks
-    // (of split products one) each.
-    const int blocks = tiles(p.K, BK) * (split ? 2 : 1);
-    while (p.splits < 8 && units(BM, 64) * 2 * p.splits <= sms() && blocks >= 4 * p.splits) p.splits *= 2;
+    // Few tiles: narrow ones (768 x 768: 89 us, with 128 x 128 106; fp32 2 x 203 x 1001: 134 and 186), and K
+    // shared by as many CTAs as fit the SMs together and have enough blocks each to pay for the exchange:
+    // 8 of single products (256 x 4096: 84 us, by twos 89; 512 x 512, not shared, 81, by twos 93), of split
+    // products one (fp32 2 x 203 x 1001: 110 us, not shared 134; 600 x 5000 278 and 444).
+    const int blocks = tiles(p.K, BK), least = split ? 1 : 8;
+    while (p.splits < 8 && units(BM, 64) * 2 * p.splits <= sms() && blocks >= 2 * least * p.splits) p.splits *= 2;
     if (p.splits > 1)
       return split ? launch_product<1, 64, true, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s)
                    : launch_product<1, 64, true, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
@@ -1142,8 +1146,23 @@ cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pa
                  : launch_product<1, 64, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
   }
   if (split) return launch_product<1, 128, false, true, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
-  // Pairs of SMs where their larger tiles still occupy half of the SMs.
-  if (tile == 2 || (tile == 0 && units(2 * BM, 2 * BM) >= sms() / 4))
+  // 128 x 128 tiles on one SM or 256 x 256 on a pair: whichever should take less time, counted in blocks
+  // of K on a pair (512 cycles).  A chain is the first tile's products, then for every further tile the
+  // longer of its products and its epilogue, then the last epilogue; a small tile has half the products
+  // and epilogue at 0.8 and 0.57 of the time (its operands are loaded 1.5 times as often), a pair 5
+  // blocks more to begin and end.  The constants are fitted to 24 shapes.  One / pairs / the rule, us
+  // for five steps: 12 x 768 x 768 200 / 222 / 200, 4 x 1024 x 1024 158 / 208 / 155, 12 x 2304 x 768
+  // 433 / 424 / 410, 1600 x 6400 420 / 436 / 370, 2500 x 2500 699 / 486 / 494, 4096 x 4096 1308 / 1106 /
+  // 1083; it errs by 3 % at 24 x 768 x 768 (377 / 349 / 366).
+  auto chain = [](long long waves, float main, float epilogue) {
+    return main + static_cast<float>(waves - 1) * fmaxf(main, epilogue) + epilogue;
+  };
+  constexpr int kPieces = MODE == kGram ? 2 : MODE == kPoly ? 3 : 4;  // 16-bit parts in and out, mirror images too
+  const float blocks = static_cast<float>(tiles(p.K, BK)), epilogue = 6.f * kPieces;
+  const int pairs = sms() / 2;
+  const float on_pairs = chain((units(2 * BM, 2 * BM) + pairs - 1) / pairs, blocks, epilogue) + 5.f;
+  const float on_one = chain((units(BM, BM) + sms() - 1) / sms(), 0.8f * blocks, 0.57f * epilogue);
+  if (tile == 2 || (tile == 0 && on_pairs <= on_one))
     return launch_product<2, 256, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
   return launch_product<1, 128, false, false, A_MN, B_MN, MODE>(a, b, c, d, p, count, s);
 }

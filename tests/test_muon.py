@@ -75,7 +75,7 @@ def test_orthogonalize(device, dtype, shape):
 @pytest.mark.gpu
 @pytest.mark.parametrize("tile", [0, 1, 2, 3])
 @pytest.mark.parametrize("shape", [(3, 70, 40), (2, 256, 256), (2, 300, 700), (3, 700, 300), (1, 1100, 1030),
-                                   (70, 40, 24)])
+                                   (70, 40, 24), (1, 100, 1100), (2, 2100, 130), (1, 200, 4200)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_tiles_and_batches(tile, shape, dtype):
     """Every tile size, and the choice, at sizes that end inside a tile, with K shared by a cluster, several

@@ -34,13 +34,13 @@
 //
 // Measured (B200; cuBLAS bf16 1634 TFLOP/s in bursts, 1395 sustained under the
 // power cap), useful operations, symmetric ones counted once: 4096 x 4096, five
-// steps, 1.09 ms = 1260 TFLOP/s in bursts, 1.33 ms = 1030 sustained (tensor pipe
+// steps, 1.09 ms = 1260 TFLOP/s in bursts, 1.32 ms = 1040 sustained (tensor pipe
 // active 76 to 82 % of the time; the rest is the last wave of 256 tiles on 74
 // pairs).  12 x 2304 x 768 with momentum and weights 465 us = 585 TFLOP/s: K is 768,
 // so a tile brings 512 KB of addend and result to 768 KB of operands (tensor pipe
 // 59 % active in X^T X, 40 % in the update).  768 x 768 89 us: 17 launches of 5.3 us,
-// each a chain of launch, first load, 12 blocks of K, of 410 cycles each at the rate
-// at which an SM takes operands from L2, and epilogue, on 42 to 72 of the SMs.
+// each a chain of launch, first load, 12 blocks of K (410 cycles each: 60 bytes of
+// operands a cycle and SM) and epilogue, on 42 to 72 of the SMs.
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 

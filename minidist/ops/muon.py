@@ -154,6 +154,12 @@ def _check_step(params, grads, momenta, shadows) -> None:
             raise ValueError(f"muon_update_: shadow {i} is not a contiguous bfloat16 {tuple(w.shape)}")
 
 
+def _check_scalar(t, name: str, device) -> None:
+    """The kernels read one float through the pointer: nothing else may stand there."""
+    if isinstance(t, torch.Tensor) and (t.numel() != 1 or t.dtype != torch.float32 or t.device != device):
+        raise ValueError(f"muon_update_: {name} {tuple(t.shape)} {t.dtype} on {t.device} is not one float32 on {device}")
+
+
 def _scale(rows: int, cols: int, rms: float) -> float:
     # An orthogonal [rows, cols] has entries of size 1 / sqrt(max(rows, cols)).
     return rms * math.sqrt(max(rows, cols))
@@ -173,13 +179,17 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     so that an update's entries have size ``lr rms`` whatever the shape (0.2 is AdamW's usual size,
     whose learning rates then carry over).  ``lr`` may be a float32 tensor of one element on the
     device.  ``shadows``: bfloat16 copies to refresh with the weights.  ``inv_scale`` / ``skip``: the
-    loss scaler's device factor on the gradients and its flag that leaves everything unchanged.
+    loss scaler's device factor on the gradients and its flag that leaves everything unchanged, each
+    one float32 on the parameters' device.  Everything is checked before anything changes.
     Matrices of one shape and device are updated together, 64 at a time."""
     _check_polynomial(steps, coefficients, eps)
     _check_step(params, grads, momenta, shadows)
     groups: dict = {}
     for i, w in enumerate(params):
         groups.setdefault((w.shape, w.device), []).append(i)
+    for device in {device for _, device in groups}:
+        for name, t in (("lr", lr), ("inv_scale", inv_scale), ("skip", skip)):
+            _check_scalar(t, name, device)
     for (shape, device), members in groups.items():
         rows, cols = shape
         if rows * cols == 0:
@@ -204,8 +214,6 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
             p.step, p.momentum, p.nesterov = 1, momentum, nesterov
             factor = _scale(rows, cols, rms)
             if isinstance(lr, torch.Tensor):
-                if lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != device:
-                    raise ValueError(f"muon_update_: lr is not one float32 on {device}")
                 p.lr, p.decay, p.rate = lr.data_ptr(), weight_decay, factor
             else:
                 p.decay, p.rate = 1.0 - lr * weight_decay, lr * factor

@@ -137,6 +137,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._check_scaler(inv_scale, skip)
         self._scaler_ptrs = (None if inv_scale is None else inv_scale.data_ptr(),
                              None if skip is None else skip.data_ptr())
         for gi, group in enumerate(self.param_groups):
@@ -204,6 +205,18 @@ class FusedAdamW(torch.optim.Optimizer):
                 denom = st["exp_avg_sq"].sqrt().div_(bc2_sqrt).add_(eps)
                 p.addcdiv_(st["exp_avg"], denom, value=-lr / bc1)
         return loss
+
+    def _check_scaler(self, *scalars: torch.Tensor | None) -> None:
+        """The update kernels read one float through each pointer: refused, before any group is
+        updated, unless that is what it points at."""
+        scalars = [t for t in scalars if t is not None]
+        if not scalars:
+            return
+        devices = {p.device for g in self.param_groups for p in g["params"] if p.is_cuda and p.grad is not None}
+        for t in scalars:
+            if t.numel() != 1 or (devices and (t.dtype != torch.float32 or devices != {t.device})):
+                raise ValueError(f"inv_scale / skip {tuple(t.shape)} {t.dtype} on {t.device} is not one float32 on the "
+                                 f"parameters' device ({', '.join(map(str, devices)) or 'cpu'})")
 
     @staticmethod
     def _wait_for(params) -> None:

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from minidist.ops import muon as M
+from minidist.optim import FusedAdamW, Muon
 
 
 def _state():
@@ -47,3 +48,30 @@ def test_scalars_that_are_taken():
         assert torch.equal(m[0], n[0]) and float((w[0] - v[0]).abs().max()) <= 2.0**-22
         M.muon_update_(w, g, m, lr=0.1, skip=torch.ones(shape))
         assert torch.equal(m[0], n[0])
+
+
+class _OnDevice(torch.nn.Parameter):
+    """A CPU parameter that says it is on a GPU, for checks that come before any launch."""
+
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("cls", [FusedAdamW, Muon])
+def test_optimizers_refuse_scalars_elsewhere(cls):
+    """Groups whose update is AdamW's kernel read the same two pointers."""
+    p = torch.nn.Parameter(torch.ones(4))
+    opt = cls([p], lr=0.1)
+    p.grad = torch.ones(4)
+    with pytest.raises(ValueError, match="inv_scale"):
+        opt.step(skip=torch.zeros(2))
+    assert torch.equal(p, torch.ones(4))
+    opt.step(skip=torch.zeros(1), inv_scale=torch.ones(1))
+    q = _OnDevice(torch.ones(4))
+    opt = cls([torch.nn.Parameter(torch.ones(4))], lr=0.1)
+    opt.param_groups[0]["params"] = [q]
+    q.grad = torch.ones(4)
+    for bad in (torch.zeros(1), torch.zeros(1, dtype=torch.bool), torch.zeros(1, dtype=torch.float64)):
+        for name in ("skip", "inv_scale"):
+            with pytest.raises(ValueError, match="cuda:0"):
+                opt.step(**{name: bad})

@@ -180,7 +180,8 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     whose learning rates then carry over).  ``lr`` may be a float32 tensor of one element on the
     device.  ``shadows``: bfloat16 copies to refresh with the weights.  ``inv_scale`` / ``skip``: the
     loss scaler's device factor on the gradients and its flag that leaves everything unchanged, each
-    one float32 on the parameters' device.  Everything is checked before anything changes.
+    one float32 on the parameters' device.  Everything is checked before anything changes.  The
+    versions of what is written go up, as with torch's own in-place operations.
     Matrices of one shape and device are updated together, 64 at a time."""
     _check_polynomial(steps, coefficients, eps)
     _check_step(params, grads, momenta, shadows)
@@ -227,3 +228,8 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
             with nat.on_device(params[part[0]]):
                 nat.check(nat.lib().md_muon(ctypes.addressof(p), nat.stream_ptr()), "md_muon")
             del workspace, held  # (reused only by later work of this stream)
+            # The kernels write through raw pointers: say so, as an in-place operation of torch's does, to
+            # autograd (saved tensors) and to whoever keeps copies by version (the fused block's bf16 weights).
+            torch.autograd.graph.increment_version([t for i in part for t in (params[i], momenta[i])])
+            if shadows is not None:
+                torch.autograd.graph.increment_version([shadows[i] for i in part if shadows[i] is not None])

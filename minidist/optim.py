@@ -375,6 +375,9 @@ class Muon(FusedAdamW):
                               coefficients=group["ns_coefficients"], rms=group["rms"], shadows=shadows,
                               inv_scale=inv_scale, skip=skip)
         if cuda:
+            for p, sh in zip(params, shadows):
+                if sh is not None:  # written with the weights: of their new version
+                    setattr(p, _SHADOW_VER, p._version)
             self._ensure_grad_buffers()
 
 

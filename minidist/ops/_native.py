@@ -169,7 +169,11 @@ def status_buffer(device: torch.device | int | None = None) -> torch.Tensor:
         idx = int(device)
     buf = _status.get(idx)
     if buf is None:
-        buf = torch.zeros(4, dtype=torch.int32, device=torch.device("cuda", idx))
+        # It outlives the mode and the stream of the call that came first.
+        with torch.inference_mode(False):
+            buf = torch.zeros(4, dtype=torch.int32, device=torch.device("cuda", idx))
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(buf.device).synchronize()
         _status[idx] = buf
     return buf
 

@@ -26,6 +26,7 @@ Two execution paths share those parameters:
 from __future__ import annotations
 
 import os
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -96,6 +97,32 @@ def _seed_for(config: GPTConfig, layer: int, role: int) -> int:
     return (config.seed * 1_000_003 + layer * 97 + role) % (2**31 - 1)
 
 
+# Tables in use, by what they hold and where: the layers of a model, and models alike, share one.
+_rotary_tables: weakref.WeakValueDictionary = weakref.WeakValueDictionary()
+
+
+def _rotary_table_of(config: GPTConfig, device: torch.device) -> tuple[torch.Tensor, bool]:
+    """The table of ``config``'s positions on ``device``, and whether it may be kept.
+
+    The first call may come from an evaluation, any stream or a graph capture, and the table outlives it:
+    made outside inference mode (an inference tensor could not be saved for a later backward) and
+    complete before it is handed out.  Inside a capture its memory would be the graph's and its
+    contents those of the last replay, so there it is part of the graph and not kept."""
+    key = (config.rotary_dim, config.block_size, config.rotary_base, config.rotary_scaling, device)
+    table = _rotary_tables.get(key)
+    if table is not None:
+        return table, True
+    capturing = device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+    with torch.inference_mode(False), torch.no_grad():
+        table = rotary_table(config.rotary_dim, config.block_size, base=config.rotary_base,
+                             scaling=config.rotary_scaling, device=device)
+    if not capturing:
+        if device.type == "cuda":
+            torch.cuda.current_stream(device).synchronize()
+        _rotary_tables[key] = table
+    return table, not capturing
+
+
 class CausalSelfAttention(nn.Module):
     """Heads sharded over the TP group: QKV column-parallel, output projection row-parallel."""
 
@@ -114,15 +141,17 @@ class CausalSelfAttention(nn.Module):
                                       group=tp_group, seed=_seed_for(config, layer, 1), device=device, dtype=dtype)
 
     def rotary(self, device) -> torch.Tensor | None:
-        """cos / sin of every position (None with learned positions); made on first use, not a parameter
-        or buffer, so checkpoints do not hold it."""
-        c = self.config
-        if c.positions != "rotary":
+        """cos / sin of every position (None with learned positions); made on first use and shared by the
+        layers, not a parameter or buffer, so checkpoints do not hold it and casts of the model leave
+        it fp32."""
+        if self.config.positions != "rotary":
             return None
-        if self._rotary is None or self._rotary.device != device:
-            self._rotary = rotary_table(c.rotary_dim, c.block_size, base=c.rotary_base, scaling=c.rotary_scaling,
-                                        device=device)
-        return self._rotary
+        if self._rotary is not None and self._rotary.device == device:
+            return self._rotary
+        table, keep = _rotary_table_of(self.config, device)
+        if keep:
+            self._rotary = table
+        return table
 
     def forward(self, x):
         B, S, _ = x.shape

@@ -76,6 +76,13 @@ def _missing_library() -> bool:
 # ---------------------------------------------------------------------------
 
 
+def _new_shadow(p: torch.Tensor) -> torch.Tensor:
+    with torch.inference_mode(False):  # refreshed later, whatever mode the first forward ran in
+        sh = torch.empty(p.shape, dtype=torch.bfloat16, device=p.device)
+    setattr(p, _SHADOW, sh)
+    return sh
+
+
 def bf16_weight(p: torch.Tensor) -> torch.Tensor:
     """bf16 view of parameter ``p`` (a cached shadow for fp32 masters, refreshed when ``p`` changes)."""
     if p.dtype == torch.bfloat16:
@@ -84,8 +91,7 @@ def bf16_weight(p: torch.Tensor) -> torch.Tensor:
     ver = p._version
     if sh is None or sh.shape != p.shape or getattr(p, _SHADOW_VER, None) != ver:
         if sh is None or sh.shape != p.shape:
-            sh = torch.empty(p.shape, dtype=torch.bfloat16, device=p.device)
-            setattr(p, _SHADOW, sh)
+            sh = _new_shadow(p)
         sh.copy_(p.detach())
         setattr(p, _SHADOW_VER, ver)
     return sh
@@ -116,8 +122,7 @@ def refresh_shadows(module: torch.nn.Module) -> None:
     for i, p in enumerate(stale):
         sh = getattr(p, _SHADOW, None)
         if sh is None or sh.shape != p.shape:
-            sh = torch.empty(p.shape, dtype=torch.bfloat16, device=p.device)
-            setattr(p, _SHADOW, sh)
+            sh = _new_shadow(p)
         ptr = p.data_ptr()
         rows.append((ptr, ptr, ptr, ptr, sh.data_ptr(), p.numel()))
         chunks += [(i, c) for c in range(-(-p.numel() // chunk))]

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from minidist.models import GPT, GPTConfig
+from minidist.models.fused_gpt import bf16_weight
 from minidist.ops import _native as nat
 from minidist.ops import muon as M
 from minidist.optim import Muon, muon_groups
@@ -85,4 +86,28 @@ def test_optimizer_keeps_its_copies_valid():
     step()
     for p in mats:
         assert p._md_bf16_ver == p._version and torch.equal(p._md_bf16, p.detach().bfloat16())
+    nat.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_copies_made_in_inference_mode_are_refreshed_outside(device):
+    p = torch.nn.Parameter(torch.randn(16, 8, device=device))
+    with torch.inference_mode():
+        bf16_weight(p)
+    with torch.no_grad():
+        p.mul_(2.0)
+    assert torch.equal(bf16_weight(p), p.detach().bfloat16())
+
+
+@pytest.mark.gpu
+def test_evaluate_in_inference_mode_then_step_one_matrix():
+    model = GPT(CFG, device="cuda")
+    ids = torch.randint(0, 1000, (2, 128), device="cuda")
+    with torch.inference_mode(), torch.autocast("cuda", dtype=torch.bfloat16):
+        model(ids)
+    w = model.blocks[0].attn.proj.weight
+    M.muon_update_([w], [torch.randn_like(w)], [torch.zeros_like(w)], lr=0.05)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        model(ids, ids)[1].backward()
+    assert torch.equal(w._md_bf16, w.detach().bfloat16())
     nat.check_status()

@@ -106,7 +106,13 @@ def _launch(q, k, q_out, k_out, table, positions, interleaved: bool, inverse: bo
 
 
 def _turn_cpu(x, table, positions, interleaved, inverse):
-    cs = table[: x.shape[1]] if positions is None else table[positions.long()]
+    if positions is None:
+        cs = table[: x.shape[1]]
+    else:
+        positions = positions.long()
+        if x.device.type == "cpu" and bool(((positions < 0) | (positions >= table.shape[0])).any()):
+            raise IndexError(f"apply_rotary: a position lies outside [0, {table.shape[0]})")
+        cs = table[positions]
     cos, sin = cs[..., 0].unsqueeze(-2), cs[..., 1].unsqueeze(-2)
     if inverse:
         sin = -sin

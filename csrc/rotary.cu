@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
   float cs[2 * NCS];
   if (pos >= 0 && pos < p.table_rows) {
     const float* t = p.table + (pos * (p.rotary / 2) + (PAIRED ? u * (HALF ? VEC : 1) : u * (VEC / 2))) * 2;
-    if (NCS % 2 == 0) {  // two entries at a time: such a vector width divides R/2, so rows are whole
+    if (NCS % 2 == 0) {  // two entries at a time: such a width divides R/2, so rows are whole and aligned
 #pragma unroll
       for (int q = 0; q < NCS / 2; ++q) {
         const float4 f = __ldg(reinterpret_cast<const float4*>(t) + q);
@@ -290,7 +290,9 @@ extern "C" int md_rotary(const MdRotaryParams* prm, cudaStream_t stream) {
   const MdRotaryParams& p = *prm;
   if (p.batch < 0 || p.seq < 0 || p.heads[0] < 0 || p.heads[1] < 0 || p.dim <= 0) return -2;
   if (p.rotary <= 0 || p.rotary % 2 || p.rotary > p.dim || p.table == nullptr || p.table_rows < 0) return -3;
-  if (reinterpret_cast<uintptr_t>(p.table) & 15u) return -4;
+  // Two entries at a time are read where a row holds an even number of them, one at a time elsewhere
+  // (an odd R/2 leaves units of one entry), so a table may start at any of its rows.
+  if (reinterpret_cast<uintptr_t>(p.table) & (p.rotary % 4 == 0 ? 15u : 7u)) return -4;
   if (p.dtype < 0 || p.dtype > 2) return -5;
   if (p.batch == 0 || p.seq == 0 || p.heads[0] + p.heads[1] == 0) return 0;
   const int es = p.dtype == 2 ? 4 : 2;

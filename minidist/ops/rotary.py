@@ -98,6 +98,8 @@ def _launch(q, k, q_out, k_out, table, positions, interleaved: bool, inverse: bo
         pos, wide, ps = positions.data_ptr(), positions.dtype == torch.int64, positions.stride()
         if len(ps) == 1:
             ps = (0, ps[0])
+    if table.data_ptr() % (8 if table.shape[1] % 2 else 16):  # (a slice of rows starts where the kernel can)
+        table = table.clone()
     params = _PARAMS.pack(q.data_ptr(), kp, q_out.data_ptr(), kop, *xs, *kxs, *ys, *kys, H, Hk, table.data_ptr(),
                           table.shape[0], pos, wide, *ps, B, S, D, 2 * table.shape[1], interleaved, inverse,
                           _DTYPE_CODE[q.dtype], nat.status_ptr(q.device))

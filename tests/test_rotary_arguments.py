@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import minidist as md
+from minidist.ops import _native as nat
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -20,3 +21,22 @@ def test_position_outside_the_table_raises_on_cpu(bad, grad):
             md.apply_rotary(q, None, table, pos)
     md.apply_rotary(q, None, table, torch.tensor([0, 7, 7, 0]))
     md.apply_rotary(q[:, :0], None, table, torch.zeros(0, dtype=torch.long))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rotary", [2, 4, 6, 10, 12, 16, 50])
+def test_table_that_starts_anywhere(device, dtype, interleaved, rotary):
+    """Rows from an offset on (to continue a sequence), and a table inside another buffer."""
+    q = torch.randn(2, 7, 3, 52, device=device).to(dtype)
+    table = md.rotary_table(rotary, 20, device=device)
+    for first in (1, 2, 3, 5):
+        want = md.apply_rotary(q, None, table, torch.arange(first, first + 7, device=device), interleaved=interleaved)[0]
+        assert torch.equal(md.apply_rotary(q, None, table[first:], interleaved=interleaved)[0], want)
+        flat = torch.zeros(first + table.numel(), device=device)
+        flat[first:] = table.flatten()
+        inside = flat[first:].view(table.shape)
+        assert torch.equal(md.apply_rotary(q, None, inside[first:], interleaved=interleaved)[0], want)
+    if device == "cuda":
+        nat.check_status()

@@ -218,4 +218,6 @@ def rotate_packed_(qkv: torch.Tensor, heads: int, table: torch.Tensor, *, batch:
     q, k = view[:, :, :, 0], view[:, :, :, 1]
     _check(q, k, table, None)
     _turn(q, k, table, None, False, inverse, inplace=True)
+    if qkv.is_cuda:  # written through a raw pointer
+        torch.autograd.graph.increment_version(qkv)
     return qkv

@@ -7,6 +7,7 @@ import torch
 
 import minidist as md
 from minidist.ops import _native as nat
+from minidist.ops import rotary as R
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -40,3 +41,15 @@ def test_table_that_starts_anywhere(device, dtype, interleaved, rotary):
         assert torch.equal(md.apply_rotary(q, None, inside[first:], interleaved=interleaved)[0], want)
     if device == "cuda":
         nat.check_status()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_turning_in_place_is_a_change_that_autograd_sees(device):
+    qkv = torch.randn(6, 3 * 2 * 16, device=device)
+    w = torch.randn(6, 3 * 2 * 16, device=device, requires_grad=True)
+    y = (w * qkv).sum()
+    version = qkv._version
+    R.rotate_packed_(qkv, 2, md.rotary_table(16, 3, device=device), batch=2)
+    assert qkv._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

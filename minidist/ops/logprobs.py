@@ -19,6 +19,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -173,7 +174,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     ``+inf`` logit makes its row's numbers NaN.  Logits may be a strided view with contiguous rows
     (the LM head's padded ones); of a tensor-parallel model gather the vocabulary first.  A token
     outside the vocabulary gives NaN, reported by :func:`minidist.ops._native.check_status` (on CPU
-    it raises).  ``top`` is at most 64.
+    it raises).  ``top`` is at most 64.  Differentiable once, in reverse mode.
     """
     if logits.dim() < 1 or logits.dtype not in _DTYPE_CODE:
         raise TypeError(f"token_logprobs: logits {tuple(logits.shape)} {logits.dtype} are not bfloat16, float16 or "
@@ -194,7 +195,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     elif flat.shape[0] <= 1 and flat.stride(0) < vocab:
         flat = flat.as_strided(flat.shape, (vocab, 1))
     ids = tokens.contiguous() if tokens.dim() == 1 else tokens.reshape(-1).contiguous()
-    need = logits.requires_grad and torch.is_grad_enabled()
+    # (A forward-mode tangent goes the same way, where torch says that there is no such derivative: a
+    # kernel launch by itself would drop it.)
+    need = (logits.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(logits).tangent is not None
     if not logits.is_cuda:
         out = _Lookup.apply(flat, ids, temperature, top, entropy, ignore_index)
     elif need:

@@ -8,7 +8,7 @@ A pair ``(a, b)`` of channels of a token at position ``p`` turns by ``p * f_i``:
 The first ``rotary_dim`` channels of each head turn, the others pass through.  On CUDA
 :func:`apply_rotary` is one sm_100a launch for queries and keys together
 (csrc/rotary.cu), on CPU the same arithmetic with torch operations; both
-differentiate (the gradient is the rotation back).
+differentiate (the gradient is the rotation back) in either mode.
 """
 
 from __future__ import annotations
@@ -18,6 +18,7 @@ import struct
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -153,7 +154,9 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, table, positions, interleaved, inverse):
         ctx.save_for_backward(table, positions)
+        ctx.save_for_forward(table, positions)
         ctx.how = (interleaved, inverse)
+        ctx.shapes = (q.shape, None if k is None else k.shape)
         ctx.set_materialize_grads(False)
         return tuple(_turn(q, k, table, positions, interleaved, inverse))
 
@@ -167,6 +170,20 @@ class _Rotary(torch.autograd.Function):
         elif dk is not None:
             dk, _ = turn(dk, None, table, positions, interleaved, not inverse)
         return dq, dk, None, None, None, None
+
+
+    @staticmethod
+    def jvp(ctx, q, k, *_):  # tangents: the operation is linear
+        table, positions = ctx.saved_tensors
+        if q is None:
+            return k.new_zeros(ctx.shapes[0]), _turn(k, None, table, positions, *ctx.how)[0]
+        turned, other = _turn(q, k, table, positions, *ctx.how)
+        return turned, q.new_zeros(ctx.shapes[1]) if k is None and ctx.shapes[1] is not None else other
+
+
+def _has_tangent(t: torch.Tensor | None) -> bool:
+    """Whether ``t`` carries a forward-mode tangent, which a kernel launch by itself would drop."""
+    return t is not None and forward_ad.unpack_dual(t).tangent is not None
 
 
 def _check(q, k, table, positions) -> None:
@@ -202,7 +219,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, p
     :func:`minidist.ops._native.check_status` (on CPU it raises).
     """
     _check(q, k, table, positions)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    grad = torch.is_grad_enabled()
+    if (grad and (q.requires_grad or (k is not None and k.requires_grad))) or _has_tangent(q) or _has_tangent(k):
         return _Rotary.apply(q, k, table, positions, interleaved, False)
     return tuple(_turn(q, k, table, positions, interleaved, False))
 

@@ -198,6 +198,8 @@ def _check(q, k, table, positions) -> None:
             or table.device != q.device or not 0 < 2 * table.shape[1] <= q.shape[3]:
         raise ValueError(f"apply_rotary: table {tuple(table.shape)} {table.dtype} is not a contiguous float32 "
                          f"[positions, rotary_dim / 2, 2] on {q.device} with rotary_dim <= {q.shape[3]}")
+    if table.requires_grad and torch.is_grad_enabled():
+        raise ValueError("apply_rotary: the table requires a gradient, but gets none (it is a constant here)")
     if positions is None:
         if q.shape[1] > table.shape[0]:
             raise ValueError(f"apply_rotary: {q.shape[1]} tokens, but the table has {table.shape[0]} positions")

@@ -53,3 +53,15 @@ def test_turning_in_place_is_a_change_that_autograd_sees(device):
     assert qkv._version > version
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_table_that_asks_for_a_gradient_is_refused(device):
+    """It would get one or none depending on the device and on whether the queries ask for theirs."""
+    table = md.rotary_table(16, 8, device=device).requires_grad_(True)
+    for grad in (False, True):
+        q = torch.randn(1, 4, 2, 16, device=device, requires_grad=grad)
+        with pytest.raises(ValueError, match="gradient"):
+            md.apply_rotary(q, None, table)
+        with torch.no_grad():
+            md.apply_rotary(q, None, table)

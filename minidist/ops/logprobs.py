@@ -29,6 +29,7 @@ nat.declare("md_logprobs", "i:pp")
 nat.declare("md_logprobs_backward", "i:pp")
 
 MAX_TOP = 64
+_COLDEST = 1e-37  # 1 / T and log2(e) / T have to be normal, finite fp32 numbers
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -185,8 +186,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
                          f"{tuple(logits.shape[:-1])} on {logits.device}")
     if vocab == 0:
         raise ValueError("token_logprobs: empty vocabulary")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"token_logprobs: temperature {temperature} is not positive and finite")
+    if not _COLDEST <= temperature <= 1.0 / _COLDEST:
+        raise ValueError(f"token_logprobs: temperature {temperature} is not within [{_COLDEST}, {1.0 / _COLDEST:g}]")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"token_logprobs: top={top} is not within [0, {min(MAX_TOP, vocab)}]")
     flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)

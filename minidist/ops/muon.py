@@ -16,6 +16,7 @@ weights in its epilogue.  On CPU the same arithmetic runs with torch operations.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from collections.abc import Sequence
 
@@ -84,6 +85,28 @@ def _check_polynomial(steps, coefficients, eps) -> None:
                          "step, three coefficients and a non-negative eps")
 
 
+@functools.lru_cache(maxsize=64)
+def _stays_in_range(steps: int, a: float, b: float, c: float) -> bool:
+    """Whether X, A = X X^T and B = b A + c A A fit the products' fp16 operands (2^12 times their
+    value, below 65504) at every step, for any matrix: singular values start within one, the
+    polynomial's largest value bounds the next step's."""
+    top = 1.0
+    for _ in range(steps):
+        values = [top * i / 1024 for i in range(1025)]
+        grams = [s * s for s in values]
+        seconds = [b * g + c * g * g for g in grams]
+        if not all(abs(v) < 15.5 for v in (top, grams[-1], *seconds)):  # (of 15.99: what rounding may add)
+            return False
+        top = max(abs(s * (a + f)) for s, f in zip(values, seconds))
+    return True
+
+
+def _check_range(steps, coefficients) -> None:
+    if not _stays_in_range(steps, *map(float, coefficients)):
+        raise ValueError(f"Newton-Schulz: coefficients={tuple(coefficients)} take singular values below one out of the "
+                         f"range of the products' operands within {steps} steps")
+
+
 def _orthogonal_cpu(u: torch.Tensor, steps, coefficients, eps) -> torch.Tensor:
     a, b, c = coefficients
     x = u.float()
@@ -124,7 +147,8 @@ def orthogonalize(u: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     one, each matrix by itself, in ``u``'s type.
 
     The polynomial ``a s + b s^3 + c s^5`` has to keep ``|s| <= 1.3`` within about two, as the default
-    and the classical ``(1.5, -0.5, 0)`` and ``(15/8, -10/8, 3/8)`` do.  bfloat16 results are within a
+    and the classical ``(1.5, -0.5, 0)`` and ``(15/8, -10/8, 3/8)`` do; one that could leave the range of
+    the kernels' operands (``s^2`` or ``b s^2 + c s^4`` of 15.5) is refused on CUDA.  bfloat16 results are within a
     bfloat16 rounding or so of exact, float16 and float32 ones within their own type's.  Not
     differentiable."""
     if u.dim() < 2 or u.dtype not in _DTYPE_CODE:
@@ -135,6 +159,7 @@ def orthogonalize(u: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
         return u.clone()
     if not u.is_cuda:
         return _orthogonal_cpu(u, steps, coefficients, eps).to(u.dtype)
+    _check_range(steps, coefficients)
     return _orthogonalize_cuda(u, steps, coefficients, eps)
 
 
@@ -191,6 +216,8 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     for device in {device for _, device in groups}:
         for name, t in (("lr", lr), ("inv_scale", inv_scale), ("skip", skip)):
             _check_scalar(t, name, device)
+        if device.type == "cuda":
+            _check_range(steps, coefficients)
     for (shape, device), members in groups.items():
         rows, cols = shape
         if rows * cols == 0:

@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import minidist as md
 from minidist.ops import muon as M
 from minidist.optim import FusedAdamW, Muon
 
@@ -75,3 +76,32 @@ def test_optimizers_refuse_scalars_elsewhere(cls):
         for name in ("skip", "inv_scale"):
             with pytest.raises(ValueError, match="cuda:0"):
                 opt.step(**{name: bad})
+
+
+def test_coefficients_that_leave_the_operands_range():
+    """fp16 operands hold X, A and B up to 15.99: what could pass that is refused, the usual ones are not."""
+    for steps, co in ((5, M.COEFFICIENTS), (100, M.COEFFICIENTS), (40, (1.5, -0.5, 0.0)), (40, (15 / 8, -10 / 8, 3 / 8)),
+                      (1, (3.0, -3.2, 1.2)), (1, (8.0, -20.0, 13.0))):
+        M._check_range(steps, co)
+    for steps, co in ((3, (4.5, -1.0, 0.0)), (2, (1.0, 4.0, 0.0)), (1, (1.0, -16.0, 0.0)), (5, (2.0, 0.0, 0.0)),
+                      (1, (1.0, float("nan"), 0.0)), (2, (float("inf"), 0.0, 0.0))):
+        with pytest.raises(ValueError, match="range"):
+            M._check_range(steps, co)
+
+
+@pytest.mark.gpu
+def test_such_coefficients_on_the_gpu():
+    u, bad = torch.randn(16, 24, device="cuda"), (2.0, 0.0, 0.0)
+    M._check_range(2, bad)
+    assert bool(md.orthogonalize(u, steps=2, coefficients=bad).isfinite().all())
+    with pytest.raises(ValueError, match="range"):
+        md.orthogonalize(u, coefficients=bad)
+    w, m = u.clone(), torch.zeros_like(u)
+    with pytest.raises(ValueError, match="range"):
+        M.muon_update_([w], [u], [m], lr=0.1, coefficients=bad)
+    assert torch.equal(w, u) and not m.any()
+    x = md.orthogonalize(u, steps=1, coefficients=(8.0, -20.0, 13.0))  # large, but held
+    v = u.double() / u.double().norm()
+    g = v @ v.t()
+    ref = 8 * v + (-20 * g + 13 * g @ g) @ v
+    assert float((x.double() - ref).norm() / ref.norm()) < 1e-4

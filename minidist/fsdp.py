@@ -86,6 +86,8 @@ class _FSDPUnit:
             flat = torch.cat([flat, flat.new_zeros(self.padded_numel - self.total_numel)])
         lo = self.rank * self.shard_numel
         self.flat_shard = nn.Parameter(flat[lo : lo + self.shard_numel].clone().to(shard_dtype))
+        for p in (self.flat_shard, *params):  # a piece of many, and views that are empty between gathers:
+            p._md_fsdp = True  # minidist.optim.Muon refuses both
         del flat
 
         self._full = torch.empty(self.padded_numel, dtype=policy.param_dtype, device=device)

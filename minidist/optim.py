@@ -21,6 +21,7 @@ learning rate from ``param_groups`` between replays.
 from __future__ import annotations
 
 import math
+import warnings
 
 import torch
 
@@ -308,13 +309,14 @@ class Muon(FusedAdamW):
     orthogonalised momentum (:func:`minidist.ops.muon.muon_update_`).  ``rms`` is the size of an
     update's entries per unit of ``lr``; 0.2, about AdamW's, lets both kinds of group share a
     learning rate.  Other groups are FusedAdamW's.  A group that does not say is orthogonal if all its
-    parameters are matrices::
+    parameters are matrices (a warning tells of matrices that a mixed one leaves to AdamW)::
 
         opt = Muon(muon_groups(model), lr=3e-4)
 
     State: ``momentum_buffer`` per matrix, AdamW's elsewhere.  Under tensor parallelism a shard is
-    orthogonalised as a matrix of its own; FSDP's flat shards are refused.  The loss scaler, deferred
-    DDP buckets and ``capturable=True`` work as with FusedAdamW.
+    orthogonalised as a matrix of its own.  FSDP's flat shards hold pieces of matrices: they are
+    refused, unless a group says ``orthogonal=False``.  The loss scaler, deferred DDP buckets and
+    ``capturable=True`` work as with FusedAdamW.
     """
 
     def __init__(self, params, lr: float = 3e-4, *, momentum: float = 0.95, nesterov: bool = True, rms: float = 0.2,
@@ -331,7 +333,12 @@ class Muon(FusedAdamW):
         params = group["params"]
         group["params"] = params = [params] if isinstance(params, torch.Tensor) else list(params)
         matrices = [p.dim() == 2 and p.dtype == torch.float32 for p in params]
-        group.setdefault("orthogonal", all(matrices))
+        if "orthogonal" not in group:
+            _refuse_flat_shards(params)
+            group["orthogonal"] = all(matrices)
+            if any(matrices) and not all(matrices):
+                warnings.warn(f"Muon: a group of {len(params)} parameters holds {sum(matrices)} matrices and others, so all "
+                              "of it takes AdamW; sort them with muon_groups(model) or say orthogonal=False", stacklevel=3)
         if group["orthogonal"]:
             if not all(matrices):
                 bad = next(p for p, ok in zip(params, matrices) if not ok)
@@ -381,10 +388,18 @@ class Muon(FusedAdamW):
             self._ensure_grad_buffers()
 
 
+def _refuse_flat_shards(params) -> None:
+    if any(getattr(p, "_md_fsdp", False) for p in params):
+        raise ValueError("Muon orthogonalises whole matrices, FSDP keeps flat shards of them: use DDP, or FusedAdamW "
+                         "for these parameters")
+
+
 def muon_groups(model: torch.nn.Module, weight_decay: float | None = None) -> list[dict]:
     """``model``'s parameters as Muon's groups: the matrices of its blocks, and (``orthogonal=False``) the
     embeddings, the LM head and everything that is not a matrix.  ``weight_decay`` applies to matrices
-    of both groups; biases and norms, a group of their own, then take none."""
+    of both groups; biases and norms, a group of their own, then take none.  A model sharded by FSDP is
+    refused."""
+    _refuse_flat_shards(model.parameters())
     hidden, tables, small = [], [], []
     for name, p in model.named_parameters():
         if not p.requires_grad:

@@ -332,6 +332,7 @@ class Muon(FusedAdamW):
     def add_param_group(self, group: dict) -> None:
         params = group["params"]
         group["params"] = params = [params] if isinstance(params, torch.Tensor) else list(params)
+        params = [p[1] if isinstance(p, tuple) else p for p in params]  # (named parameters)
         matrices = [p.dim() == 2 and p.dtype == torch.float32 for p in params]
         if "orthogonal" not in group:
             _refuse_flat_shards(params)

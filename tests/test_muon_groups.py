@@ -45,3 +45,16 @@ def test_a_mixed_group_says_what_it_leaves_to_adamw():
         Muon([vec])
         Muon([dict(params=[vec, mat], orthogonal=False)])
         Muon(muon_groups(GPT(CFG)))
+
+
+def test_named_parameters():
+    lin = torch.nn.Linear(3, 4)
+    opt = Muon([dict(params=[("weight", lin.weight)]), dict(params=[("bias", lin.bias)])], lr=0.1)
+    assert [g["orthogonal"] for g in opt.param_groups] == [True, False]
+    assert opt.param_groups[0]["param_names"] == ["weight"]
+    before = lin.weight.detach().clone()
+    lin(torch.randn(2, 3)).sum().backward()
+    opt.step()
+    assert not torch.equal(before, lin.weight) and "momentum_buffer" in opt.state[lin.weight]
+    with pytest.warns(UserWarning, match="takes AdamW"):
+        Muon(lin.named_parameters())

@@ -97,7 +97,8 @@ def parse_args(argv=None) -> argparse.Namespace:
                           "updates for the blocks' matrices, fused AdamW for the rest")
     run.add_argument("--score-every", type=int, default=0, metavar="N",
                      help="every N steps print the mean log probability and entropy of the batch's targets and "
-                          "how often a target is among the 5 likeliest tokens (no pipeline, no tensor parallelism)")
+                          "how often a target is among the 5 likeliest tokens, outside the timing (no pipeline, no tensor "
+                          "parallelism)")
     run.add_argument("--timing", default="auto", choices=["auto", "device", "host"])
     run.add_argument("--save", metavar="DIR", default=None, help="write a checkpoint here at the end")
     run.add_argument("--kernels", default="fused", choices=["fused", "nccl"],
@@ -310,26 +311,36 @@ def main(argv=None) -> None:
         ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         ev0.record()
     start = time.perf_counter()
+    scoring, score_events = 0.0, []  # time spent on scores is not the training's
     for step in range(1, args.steps + 1):
         loss = train_step(step)
         if step % max(1, args.steps // 10) == 0:
-            el = time.perf_counter() - start
+            el = time.perf_counter() - start - scoring
             print_rank0(f"  step {step:>4}/{args.steps}  loss {loss:>7.4f}  {el / step * 1e3:>7.1f} ms/step  "
                         f"{tokens_per_step * step / el:>9.0f} tok/s")
             metrics.write(step=step, loss=loss, ms_per_step=el / step * 1e3, tokens_per_s=tokens_per_step * step / el,
                           timing="host, rank 0")
         if args.score_every and step % args.score_every == 0:
+            if device.type == "cuda":
+                torch.cuda.synchronize()  # the step's own work ends here
+            if device_timing:
+                score_events.append([torch.cuda.Event(enable_timing=True) for _ in range(2)])
+                score_events[-1][0].record()
+            paused = time.perf_counter()
             s = score(step)
             print_rank0(f"  step {step:>4}/{args.steps}  targets: mean log p {s['logprob']:.4f}  entropy "
                         f"{s['entropy']:.4f}  among the five likeliest {100 * s['top5']:.2f}%")
             metrics.write(event="score", step=step, **s)
+            scoring += time.perf_counter() - paused
+            if device_timing:
+                score_events[-1][1].record()
     if device.type == "cuda":
         torch.cuda.synchronize()
-    total = time.perf_counter() - start
+    total = time.perf_counter() - start - scoring
     if device_timing:
         ev1.record()
         ev1.synchronize()
-        total = ev0.elapsed_time(ev1) / 1e3
+        total = (ev0.elapsed_time(ev1) - sum(a.elapsed_time(b) for a, b in score_events)) / 1e3
     total = _max_over_ranks(total, device)
     kind = "device time, max over ranks" if device_timing else "host time, max over ranks"
     print_rank0(f"\n  {args.steps} steps in {total:.2f}s ({total / args.steps * 1e3:.1f} ms/step, "

@@ -119,14 +119,14 @@ def _orthogonal_cpu(u: torch.Tensor, steps, coefficients, eps) -> torch.Tensor:
     return x.mT if tall else x
 
 
-def _orthogonalize_cuda(u: torch.Tensor, steps, coefficients, eps, tile: int = 0) -> torch.Tensor:
+def _orthogonalize_cuda(u: torch.Tensor, steps, coefficients, eps, tile: int = 0, precise: bool = False) -> torch.Tensor:
     rows, cols = u.shape[-2:]
     u = u.contiguous()
     out = torch.empty_like(u)
     count = u.numel() // (rows * cols)
     # A bf16 answer is rounded more coarsely than one product of fp16 parts errs; fp16 and fp32
     # answers take the three-product form.
-    split = u.dtype != torch.bfloat16
+    split = precise or u.dtype != torch.bfloat16
     size = rows * cols * u.element_size()
     for at in range(0, count, _BATCH):
         n = min(_BATCH, count - at)
@@ -142,15 +142,16 @@ def _orthogonalize_cuda(u: torch.Tensor, steps, coefficients, eps, tile: int = 0
 
 
 def orthogonalize(u: torch.Tensor, *, steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS,
-                  eps: float = 1e-7) -> torch.Tensor:
+                  eps: float = 1e-7, precise: bool = False) -> torch.Tensor:
     """``u [..., rows, cols]`` (bfloat16, float16 or float32) with its singular values driven towards
     one, each matrix by itself, in ``u``'s type.
 
     The polynomial ``a s + b s^3 + c s^5`` has to keep ``|s| <= 1.3`` within about two, as the default
     and the classical ``(1.5, -0.5, 0)`` and ``(15/8, -10/8, 3/8)`` do; one that could leave the range of
     the kernels' operands (``s^2`` or ``b s^2 + c s^4`` of 15.5) is refused on CUDA.  bfloat16 results are within a
-    bfloat16 rounding or so of exact, float16 and float32 ones within their own type's.  Not
-    differentiable."""
+    bfloat16 rounding or so of exact, float16 and float32 ones within their own type's; ``precise``
+    takes those types' products (three of fp16 parts each instead of one) for bfloat16 as well, whose
+    results are then off by their rounding alone.  Not differentiable."""
     if u.dim() < 2 or u.dtype not in _DTYPE_CODE:
         raise TypeError(f"orthogonalize: {tuple(u.shape)} {u.dtype} is not a bfloat16, float16 or float32 matrix")
     _check_polynomial(steps, coefficients, eps)
@@ -160,7 +161,7 @@ def orthogonalize(u: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
     if not u.is_cuda:
         return _orthogonal_cpu(u, steps, coefficients, eps).to(u.dtype)
     _check_range(steps, coefficients)
-    return _orthogonalize_cuda(u, steps, coefficients, eps)
+    return _orthogonalize_cuda(u, steps, coefficients, eps, precise=precise)
 
 
 def _check_step(params, grads, momenta, shadows) -> None:
@@ -190,12 +191,43 @@ def _scale(rows: int, cols: int, rms: float) -> float:
     return rms * math.sqrt(max(rows, cols))
 
 
+def _step_cuda(params, grads, momenta, shadows, lr, momentum, nesterov, weight_decay, steps, coefficients, eps, rms,
+               inv_scale, skip, precise, tile: int = 0) -> None:
+    """Up to ``_BATCH`` equally shaped matrices of one device, checked by the caller."""
+    n, device = len(params), params[0].device
+    rows, cols = params[0].shape
+    # One product of fp16 parts, unless asked otherwise: X errs by 1e-3 or 2e-3 of itself, and the weights
+    # take lr rms of it.
+    p, workspace = _params(n, rows, cols, _DTYPE_CODE[torch.float32], precise, steps, coefficients, eps, device)
+    p.tile, p.step, p.momentum, p.nesterov = tile, 1, momentum, nesterov
+    factor = _scale(rows, cols, rms)
+    if isinstance(lr, torch.Tensor):
+        p.lr, p.decay, p.rate = lr.data_ptr(), weight_decay, factor
+    else:
+        p.decay, p.rate = 1.0 - lr * weight_decay, lr * factor
+    p.inv_scale, p.skip = nat.ptr(inv_scale), nat.ptr(skip)
+    held = [g.contiguous() for g in grads]
+    p.src[:n] = [g.data_ptr() for g in held]
+    p.m[:n] = [m.data_ptr() for m in momenta]
+    p.out[:n] = [w.data_ptr() for w in params]
+    if shadows is not None:
+        p.shadow[:n] = [nat.ptr(sh) for sh in shadows]
+    with nat.on_device(params[0]):
+        nat.check(nat.lib().md_muon(ctypes.addressof(p), nat.stream_ptr()), "md_muon")
+    del workspace, held  # (reused only by later work of this stream)
+    # The kernels write through raw pointers: say so, as an in-place operation of torch's does, to
+    # autograd (saved tensors) and to whoever keeps copies by version (the fused block's bf16 weights).
+    torch.autograd.graph.increment_version([*params, *momenta])
+    if shadows is not None:
+        torch.autograd.graph.increment_version([sh for sh in shadows if sh is not None])
+
+
 @torch.no_grad()
 def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], *,
                  lr: float | torch.Tensor, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  steps: int = 5, coefficients: Sequence[float] = COEFFICIENTS, eps: float = 1e-7, rms: float = 0.2,
                  shadows: Sequence[torch.Tensor | None] | None = None, inv_scale: torch.Tensor | None = None,
-                 skip: torch.Tensor | None = None) -> None:
+                 skip: torch.Tensor | None = None, precise: bool = False) -> None:
     """One Muon step on fp32 matrices, in place::
 
         m = momentum m + g        u = g + momentum m  (m without nesterov)
@@ -207,7 +239,11 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     loss scaler's device factor on the gradients and its flag that leaves everything unchanged, each
     one float32 on the parameters' device.  Everything is checked before anything changes.  The
     versions of what is written go up, as with torch's own in-place operations.
-    Matrices of one shape and device are updated together, 64 at a time."""
+    Matrices of one shape and device are updated together, 64 at a time.
+
+    On CUDA an update comes from single products of fp16 parts and is off by about 2e-3 of itself;
+    ``precise`` takes three products, as for a float32 :func:`orthogonalize`: off by 1e-5 or less, in 2.1
+    to 2.7 times the time (12 x 2304 x 768 469 and 1061 us, 1600 x 6400 396 and 1077)."""
     _check_polynomial(steps, coefficients, eps)
     _check_step(params, grads, momenta, shadows)
     groups: dict = {}
@@ -236,27 +272,6 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
             continue
         for at in range(0, len(members), _BATCH):
             part = members[at: at + _BATCH]
-            n = len(part)
-            # One product of fp16 parts: X errs by 1e-3 of itself, and the weights take lr rms of it.
-            p, workspace = _params(n, rows, cols, 2, False, steps, coefficients, eps, device)
-            p.step, p.momentum, p.nesterov = 1, momentum, nesterov
-            factor = _scale(rows, cols, rms)
-            if isinstance(lr, torch.Tensor):
-                p.lr, p.decay, p.rate = lr.data_ptr(), weight_decay, factor
-            else:
-                p.decay, p.rate = 1.0 - lr * weight_decay, lr * factor
-            p.inv_scale, p.skip = nat.ptr(inv_scale), nat.ptr(skip)
-            held = [grads[i].contiguous() for i in part]
-            p.src[:n] = [g.data_ptr() for g in held]
-            p.m[:n] = [momenta[i].data_ptr() for i in part]
-            p.out[:n] = [params[i].data_ptr() for i in part]
-            if shadows is not None:
-                p.shadow[:n] = [nat.ptr(shadows[i]) for i in part]
-            with nat.on_device(params[part[0]]):
-                nat.check(nat.lib().md_muon(ctypes.addressof(p), nat.stream_ptr()), "md_muon")
-            del workspace, held  # (reused only by later work of this stream)
-            # The kernels write through raw pointers: say so, as an in-place operation of torch's does, to
-            # autograd (saved tensors) and to whoever keeps copies by version (the fused block's bf16 weights).
-            torch.autograd.graph.increment_version([t for i in part for t in (params[i], momenta[i])])
-            if shadows is not None:
-                torch.autograd.graph.increment_version([shadows[i] for i in part if shadows[i] is not None])
+            _step_cuda(*([t[i] for i in part] for t in (params, grads, momenta)),
+                       None if shadows is None else [shadows[i] for i in part], lr, momentum, nesterov, weight_decay,
+                       steps, coefficients, eps, rms, inv_scale, skip, precise)

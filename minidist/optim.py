@@ -308,8 +308,9 @@ class Muon(FusedAdamW):
     ``w = (1 - lr weight_decay) w - lr rms sqrt(max(rows, cols)) X`` where ``X`` is the
     orthogonalised momentum (:func:`minidist.ops.muon.muon_update_`).  ``rms`` is the size of an
     update's entries per unit of ``lr``; 0.2, about AdamW's, lets both kinds of group share a
-    learning rate.  Other groups are FusedAdamW's.  A group that does not say is orthogonal if all its
-    parameters are matrices (a warning tells of matrices that a mixed one leaves to AdamW)::
+    learning rate.  ``precise`` takes products of fp32's precision on CUDA.  Other groups are
+    FusedAdamW's.  A group that does not say is orthogonal if all its parameters are matrices (a warning
+    tells of matrices that a mixed one leaves to AdamW)::
 
         opt = Muon(muon_groups(model), lr=3e-4)
 
@@ -321,12 +322,12 @@ class Muon(FusedAdamW):
 
     def __init__(self, params, lr: float = 3e-4, *, momentum: float = 0.95, nesterov: bool = True, rms: float = 0.2,
                  ns_steps: int = 5, ns_coefficients=muon_ops.COEFFICIENTS, betas=(0.9, 0.95), eps: float = 1e-8,
-                 weight_decay: float = 1e-2, capturable: bool = False):
+                 weight_decay: float = 1e-2, capturable: bool = False, precise: bool = False):
         if not 0 <= momentum < 1 or not rms > 0 or ns_steps < 1 or len(ns_coefficients) != 3:
             raise ValueError("invalid Muon hyper-parameters")
         # add_param_group (called by the base constructor) completes each group from these
         self._matrix_defaults = dict(momentum=momentum, nesterov=nesterov, rms=rms, ns_steps=ns_steps,
-                                     ns_coefficients=tuple(ns_coefficients))
+                                     ns_coefficients=tuple(ns_coefficients), precise=precise)
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable)
 
     def add_param_group(self, group: dict) -> None:
@@ -381,7 +382,7 @@ class Muon(FusedAdamW):
                               [self.state[p]["momentum_buffer"] for p in params], lr=lr, momentum=group["momentum"],
                               nesterov=group["nesterov"], weight_decay=group["weight_decay"], steps=group["ns_steps"],
                               coefficients=group["ns_coefficients"], rms=group["rms"], shadows=shadows,
-                              inv_scale=inv_scale, skip=skip)
+                              inv_scale=inv_scale, skip=skip, precise=group.get("precise", False))
         if cuda:
             for p, sh in zip(params, shadows):
                 if sh is not None:  # written with the weights: of their new version

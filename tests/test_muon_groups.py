@@ -58,3 +58,15 @@ def test_named_parameters():
     assert not torch.equal(before, lin.weight) and "momentum_buffer" in opt.state[lin.weight]
     with pytest.warns(UserWarning, match="takes AdamW"):
         Muon(lin.named_parameters())
+
+
+def test_precise_is_kept_with_the_group():
+    mats = [torch.nn.Parameter(torch.randn(4, 6)) for _ in range(2)]
+    opt = Muon([dict(params=[mats[0]], precise=True), dict(params=[mats[1]])])
+    assert [g["precise"] for g in opt.param_groups] == [True, False]
+    saved = opt.state_dict()
+    del saved["param_groups"][1]["precise"]  # a state from before the option
+    opt.load_state_dict(saved)
+    for p in mats:
+        p.grad = torch.ones_like(p)
+    opt.step()

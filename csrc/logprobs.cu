@@ -91,6 +91,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
 
+// Terms of sums that hold a 1 (the row's maximum), and p itself: 2 ulp, and 0 below 2^-126, are far
+// under the 2^-24 that each of a lane's additions costs, and it is one instruction where the exact
+// function is several in a loop whose issue slots are two thirds full.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -679,7 +682,8 @@ template <typename T, bool ENT, bool TOP>
 cudaError_t launch_forward(const MdLogprobsParams& p, cudaStream_t stream) {
   const int nv = p.vocab / Pack<T>::N;
   // Sums alone: the fewest warps per row that keep the SMs full (a warp's joins and tail cost less
-  // the longer its share; 8192 rows of 50257: 138 us with one warp each, 166 us with four).  With
+  // the longer its share; 8192 rows of 50257 bf16: 147 us with one warp each, 138 with two, as here,
+  // 142 with four; 6000 rows 127, 111, 108; 8192 rows of 8192 29, 31, 40).  With
   // alternatives a block, whose selection runs under the reads of the others on its SM, or a warp for
   // rows too short for that (2000 rows of 8192, top 32: 23 us with blocks, 26 us with warps; 8192
   // rows of 1000, top 5: 19 us with warps, 51 us with blocks).

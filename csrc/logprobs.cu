@@ -91,9 +91,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
 
-// Terms of sums that hold a 1 (the row's maximum), and p itself: 2 ulp, and 0 below 2^-126, are far
-// under the 2^-24 that each of a lane's additions costs, and it is one instruction where the exact
-// function is several in a loop whose issue slots are two thirds full.
+// Terms of sums that hold a 1 (the row's maximum), and p itself: 2 ulp, and 0 below 2^-126, are under
+// what a lane's hundreds of additions at 2^-24 each may cost, and this is one instruction where the
+// exact function is several, in a loop whose issue slots are two thirds full.
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -152,7 +152,7 @@ struct MdEmbTpParams {
   unsigned long long timeout_ns;
   md::Status* status;
   const long long* ids;       // [M] token ids (global vocabulary)
-  const __nv_bfloat16* wpe;   // [>= S, ldp] position rows (local)
+  const __nv_bfloat16* wpe;   // [>= S, ldp] position rows (local), or null: none are added
   long long ldp;
   __nv_bfloat16* out;         // [M, ldo]
   long long ldo;
@@ -526,7 +526,8 @@ __global__ void __launch_bounds__(256) md_embed_tp_kernel(const __grid_constant_
       const bool valid = id >= 0 && row < p.vocab_rows;
       MD_CHECK(valid, p.status, 142, id);  // an id outside the vocabulary reads as a zero row
       const uint4* src = reinterpret_cast<const uint4*>(p.wte[valid ? owner : 0] + (valid ? row : 0) * p.ldw);
-      const uint4* pos = reinterpret_cast<const uint4*>(p.wpe + static_cast<long long>(m % p.S) * p.ldp);
+      const uint4* pos =
+          p.wpe == nullptr ? nullptr : reinterpret_cast<const uint4*>(p.wpe + static_cast<long long>(m % p.S) * p.ldp);
       uint4* dst = reinterpret_cast<uint4*>(p.out + static_cast<long long>(m) * p.ldo);
       for (int j0 = lane; j0 < nvec; j0 += 32 * U) {
         uint4 w[U];
@@ -539,6 +540,10 @@ __global__ void __launch_bounds__(256) md_embed_tp_kernel(const __grid_constant_
         for (int k = 0; k < U; ++k) {
           const int j = j0 + 32 * k;
           if (j >= nvec) break;
+          if (p.wpe == nullptr) {
+            dst[j] = w[k];
+            continue;
+          }
           const uint4 q = pos[j];
           const uint32_t a[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
           const uint32_t b[4] = {q.x, q.y, q.z, q.w};
@@ -566,7 +571,7 @@ extern "C" {
 int md_embed_tp(const MdEmbTpParams* prm, int ctas, cudaStream_t s) {
   if (prm == nullptr || prm->world < 1 || prm->world > md::symm::kMaxWorld || prm->M <= 0 || prm->S <= 0 ||
       prm->C <= 0 || (prm->C % 8) || (prm->ldw % 8) || (prm->ldp % 8) || (prm->ldo % 8) || prm->vocab_rows <= 0 ||
-      prm->out == nullptr || prm->ids == nullptr || prm->wpe == nullptr)
+      prm->out == nullptr || prm->ids == nullptr)
     return -1;
   if (ctas < 1 || ctas > md::symm::kMaxCtas || prm->channel < 0 || prm->channel >= md::symm::kChannels) return -2;
   md::symm::md_embed_tp_kernel<<<ctas, 256, 0, s>>>(*prm);

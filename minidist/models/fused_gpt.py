@@ -254,14 +254,15 @@ class _EmbeddingFn(torch.autograd.Function):
         group = emb.group
         tp = _tp_world(group)
         x = None
-        if tp > 1 and wpe is not None:
+        pos = None if wpe is None else bf16_weight(wpe)[:S]
+        if tp > 1:
             from ..parallel import collectives
 
             # Each row read from the rank that owns its vocabulary range (no reduction).
-            x = collectives.embedding_tp(ids, wte, bf16_weight(wpe)[:S], group)
+            x = collectives.embedding_tp(ids, wte, pos, group)
         if x is None:
-            add_pos = wpe is not None and (tp == 1 or emb.rank == 0)  # positions summed once across the TP reduction
-            x = K.embedding_fwd(ids, bf16_weight(wte), bf16_weight(wpe)[:S] if add_pos else None, S,
+            add_pos = tp == 1 or emb.rank == 0  # positions summed once across the TP reduction
+            x = K.embedding_fwd(ids, bf16_weight(wte), pos if add_pos else None, S,
                                 vocab_start=emb.vocab_start if tp > 1 else 0)
             if tp > 1:
                 _all_reduce_(x, group)

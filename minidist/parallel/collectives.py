@@ -210,8 +210,8 @@ def symmetric_bf16_shadow(c: symm.Communicator, p: torch.Tensor):
     return F.bf16_weight(p), buf
 
 
-def embedding_tp(ids: torch.Tensor, wte: torch.Tensor, wpe_bf16: torch.Tensor, group) -> torch.Tensor | None:
-    """Vocab-parallel embedding forward ``wte[ids] + wpe[s]`` (bf16 ``[B*S, C]``) read straight from
+def embedding_tp(ids: torch.Tensor, wte: torch.Tensor, wpe_bf16: torch.Tensor | None, group) -> torch.Tensor | None:
+    """Vocab-parallel embedding forward ``wte[ids] (+ wpe[s])`` (bf16 ``[B*S, C]``) read straight from
     the owning rank's table shard over NVLink (``md_embed_tp``); ``None`` when peer memory is
     unavailable for ``group`` (the caller does the masked lookup + NCCL all-reduce)."""
     if not _tp_fused_enabled() or wte.dtype != torch.float32:
@@ -231,7 +231,9 @@ def embedding_tp(ids: torch.Tensor, wte: torch.Tensor, wpe_bf16: torch.Tensor, g
         prm.wte[r], prm.flags[r] = buf.ptrs[r], buf.flag_ptrs[r]
     prm.world, prm.rank, prm.channel = c.world, c.rank, _EMB_CHANNEL
     prm.timeout_ns, prm.status = _timeout_ns(), nat.status_ptr(ids.device)
-    prm.ids, prm.wpe, prm.ldp = ids_c.data_ptr(), wpe_bf16.data_ptr(), wpe_bf16.stride(0)
+    prm.ids = ids_c.data_ptr()
+    if wpe_bf16 is not None:
+        prm.wpe, prm.ldp = wpe_bf16.data_ptr(), wpe_bf16.stride(0)
     prm.out, prm.ldo = out.data_ptr(), out.stride(0)
     prm.ldw, prm.vocab_rows = shadow.stride(0), shadow.shape[0]
     prm.M, prm.S, prm.C = M, S, C

@@ -277,7 +277,9 @@ class FusedAdamW(torch.optim.Optimizer):
         rows, key = [], []
         for p in params:
             st = self.state[p]
-            g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
+            if not p.grad.is_contiguous():  # (kept: the kernel reads it through the table)
+                p.grad = p.grad.contiguous()
+            g = p.grad
             sh = getattr(p, _SHADOW, None)
             if sh is not None and (sh.shape != p.shape or getattr(p, _SHADOW_VER, None) != p._version):
                 sh = None  # stale shadow: let the next forward recast it

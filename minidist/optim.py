@@ -105,14 +105,17 @@ class FusedAdamW(torch.optim.Optimizer):
             params = [p for p in group["params"] if p.grad is not None]
             if group.get("orthogonal"):
                 self._wait_for(params)
-                for p in params:
-                    flag.add_((~torch.isfinite(p.grad)).any().to(flag.dtype).to(flag.device))
-                continue
             fused = [p for p in params if p.is_cuda and p.dtype == torch.float32 and p.grad.dtype == torch.float32]
             fused_ids = {id(p) for p in fused}
             for p in params:
                 if id(p) not in fused_ids:
                     flag.add_((~torch.isfinite(p.grad)).any().to(flag.dtype).to(flag.device))
+            if group.get("orthogonal"):
+                if fused:
+                    table, chunk_t, n = self._table(("grads", gi), fused, moments=False)
+                    nat.check(nat.lib().md_nonfinite(table.data_ptr(), chunk_t.data_ptr(), n, flag.data_ptr(),
+                                                     nat.stream_ptr()), "md_nonfinite")
+                continue
             self._init_states(fused)  # the kernel table points at the moments too
             if fused:
                 for key, part in self._partitions(gi, fused):
@@ -268,23 +271,23 @@ class FusedAdamW(torch.optim.Optimizer):
             if getattr(p, _SHADOW, None) is not None:
                 setattr(p, "_md_bf16_ver", p._version)
 
-    def _table(self, gi, params):
+    def _table(self, gi, params, moments: bool = True):
         """Device (tensor, chunk) table of ``params`` for the multi-tensor kernels, cached per key
-        while the pointers stay the same."""
+        while the pointers stay the same (``moments=False``: for passes over the gradients alone)."""
         from .models.fused_gpt import _SHADOW, _SHADOW_VER
 
         lib = nat.lib()
         rows, key = [], []
         for p in params:
-            st = self.state[p]
+            st = self.state[p] if moments else None
             if not p.grad.is_contiguous():  # (kept: the kernel reads it through the table)
                 p.grad = p.grad.contiguous()
             g = p.grad
             sh = getattr(p, _SHADOW, None)
             if sh is not None and (sh.shape != p.shape or getattr(p, _SHADOW_VER, None) != p._version):
                 sh = None  # stale shadow: let the next forward recast it
-            ptrs = (p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(),
-                    sh.data_ptr() if sh is not None else 0, p.numel())
+            m, v = (st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()) if moments else (0, 0)
+            ptrs = (p.data_ptr(), g.data_ptr(), m, v, sh.data_ptr() if sh is not None else 0, p.numel())
             rows.append(ptrs)
             key.append(ptrs)
         key = tuple(key)

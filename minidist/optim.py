@@ -260,16 +260,13 @@ class FusedAdamW(torch.optim.Optimizer):
         self._grad_flat = flat
 
     def _fused_update(self, gi, params, lr, b1, b2, eps, wd, bc1, bc2_sqrt, hp=None) -> None:
-        from .models.fused_gpt import _SHADOW
-
         table, chunk_t, n = self._table(gi, params)
         inv_ptr, skip_ptr = getattr(self, "_scaler_ptrs", (None, None))
         rc = nat.lib().md_adamw(table.data_ptr(), chunk_t.data_ptr(), n, lr, b1, b2, eps, wd, bc1, bc2_sqrt,
                                 inv_ptr, skip_ptr, 0, nat.stream_ptr(), None if hp is None else hp.data_ptr())
         nat.check(rc, "md_adamw")
-        for p in params:
-            if getattr(p, _SHADOW, None) is not None:
-                setattr(p, "_md_bf16_ver", p._version)
+        # (The kernel leaves the versions as they are, so the bf16 copies that it refreshed stay valid, and
+        # those that it was not given because they were stale stay stale.)
 
     def _table(self, gi, params, moments: bool = True):
         """Device (tensor, chunk) table of ``params`` for the multi-tensor kernels, cached per key

@@ -232,6 +232,9 @@ def main(argv=None) -> None:
 
     if args.optimizer == "muon" and args.strategy == "fsdp" and mesh.dp_size > 1:
         raise SystemExit("--optimizer muon needs whole matrices: FSDP keeps flat shards of them")
+    if args.optimizer == "muon" and mesh.tp_size > 1:
+        print_rank0(f"  muon: each of the {mesh.tp_size} tensor-parallel shards of a matrix is orthogonalised as a matrix "
+                    "of its own, so updates depend on --tp")
     if args.score_every and (mesh.pp_size > 1 or mesh.tp_size > 1):
         raise SystemExit("--score-every needs the whole model and vocabulary on every rank (pp = tp = 1)")
     model, core, loss_fn = build(args, mesh, config, device, precision)

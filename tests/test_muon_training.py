@@ -3,6 +3,10 @@
 from __future__ import annotations
 
 import copy
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -133,3 +137,16 @@ def _tensor_parallel(rank, world):
 @pytest.mark.parametrize("world", [2, 4])
 def test_rotary_under_tensor_parallelism(world):
     run_distributed(_tensor_parallel, world)
+
+
+def test_trainer_says_that_updates_depend_on_tp():
+    root = Path(__file__).resolve().parent.parent
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--master-addr=127.0.0.1"]
+    args = ["--layers", "1", "--embd", "32", "--heads", "2", "--vocab", "64", "--seq-len", "16", "--batch-size", "2", "--steps",
+            "1", "--backend", "gloo", "--optimizer", "muon"]
+    for tp in (1, 2):
+        proc = subprocess.run([*cmd, "--nproc-per-node=2", "--master-port=29583", str(root / "examples" / "train_gpt.py"), *args,
+                               "--tp", str(tp)], capture_output=True, text=True, timeout=300, cwd=root,
+                              env=dict(os.environ, OMP_NUM_THREADS="1", CUDA_VISIBLE_DEVICES=""))
+        assert proc.returncode == 0, proc.stderr[-3000:]
+        assert ("updates depend on --tp" in proc.stdout) == (tp > 1)

@@ -418,9 +418,15 @@ __device__ __forceinline__ void select(const Share<T>& sh, const float (&top)[kP
   sync();
 }
 
+// Blocks per SM that the registers are cut for: ten (48 registers), eight (64) for fp32 logits with
+// alternatives, which at 48 spill 164 bytes in the loop (2048 x 50257, top 5: 78 us with eight, 80 with
+// nine, 83 with ten; without entropy 77, 80, 90).
+template <typename T, bool TOP>
+constexpr int kBlocksPerSm = TOP && sizeof(T) == 4 ? 8 : 10;
+
 // `share` warps per row (1, 2 or 4), or with ctas > 1 whole blocks of a cluster.
 template <typename T, bool ENT, bool TOP>
-__global__ void __launch_bounds__(kThreads, 10) forward_kernel(const __grid_constant__ MdLogprobsParams p, int share, int ctas) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm<T, TOP>) forward_kernel(const __grid_constant__ MdLogprobsParams p, int share, int ctas) {
   constexpr int N = Pack<T>::N;
   constexpr uint32_t kFull = 0xFFFFFFFFu;
   extern __shared__ __align__(16) uint8_t smem_raw[];

@@ -31,6 +31,7 @@ nat.declare("md_muon_workspace", "l:iiii")
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _BATCH = 64
+_WORKSPACE = 4 << 30  # bytes at most, unless one matrix takes more
 _DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -77,6 +78,13 @@ def _params(count, rows, cols, dtype, split, steps, coefficients, eps, device):
     p.workspace, p.workspace_bytes = workspace.data_ptr(), size
     p.status = nat.status_ptr(device)
     return p, workspace
+
+
+def _per_call(rows: int, cols: int, split) -> int:
+    """Matrices updated together: batches are for small ones, whose tiles do not fill the SMs one by one,
+    and their workspace (both parts of X twice, A and B) must not grow with a large model (six of
+    16384 x 4096 take 22 to 25 ms whether by 1, by 3 or together, and 0.6, 1.7 or 3.4 GiB)."""
+    return max(1, min(_BATCH, _WORKSPACE // max(1, nat.lib().md_muon_workspace(1, rows, cols, split))))
 
 
 def _check_polynomial(steps, coefficients, eps) -> None:
@@ -128,8 +136,9 @@ def _orthogonalize_cuda(u: torch.Tensor, steps, coefficients, eps, tile: int = 0
     # answers take the three-product form.
     split = precise or u.dtype != torch.bfloat16
     size = rows * cols * u.element_size()
-    for at in range(0, count, _BATCH):
-        n = min(_BATCH, count - at)
+    together = _per_call(rows, cols, split)
+    for at in range(0, count, together):
+        n = min(together, count - at)
         p, workspace = _params(n, rows, cols, _DTYPE_CODE[u.dtype], split, steps, coefficients, eps, u.device)
         p.tile = tile
         src, dst = u.data_ptr() + at * size, out.data_ptr() + at * size
@@ -239,7 +248,7 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     loss scaler's device factor on the gradients and its flag that leaves everything unchanged, each
     one float32 on the parameters' device.  Everything is checked before anything changes.  The
     versions of what is written go up, as with torch's own in-place operations.
-    Matrices of one shape and device are updated together, 64 at a time.
+    Matrices of one shape and device are updated together, up to 64 and 4 GiB of workspace at a time.
 
     On CUDA an update comes from single products of fp16 parts and is off by about 2e-3 of itself;
     ``precise`` takes three products, as for a float32 :func:`orthogonalize`: off by 1e-5 or less, in 2.1
@@ -270,8 +279,9 @@ def muon_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
                 if shadows is not None and shadows[i] is not None:
                     shadows[i].copy_(params[i])
             continue
-        for at in range(0, len(members), _BATCH):
-            part = members[at: at + _BATCH]
+        together = _per_call(rows, cols, precise)
+        for at in range(0, len(members), together):
+            part = members[at: at + together]
             _step_cuda(*([t[i] for i in part] for t in (params, grads, momenta)),
                        None if shadows is None else [shadows[i] for i in part], lr, momentum, nesterov, weight_decay,
                        steps, coefficients, eps, rms, inv_scale, skip, precise)

@@ -225,6 +225,7 @@ __global__ void __launch_bounds__(kThreads) convert_kernel(const __grid_constant
 // ---------------------------------------------------------------------------
 constexpr int BM = 128;   // rows of A per CTA and stage
 constexpr int BK = 64;
+constexpr int kShort = 128;  // K up to this: split products fill an accumulator for every 16 of it
 constexpr int kOperand = BM * BK * 2;  // 16 KB
 constexpr int kRing = 10 * kOperand;   // shared memory for the stages (and the partial sums of a shared K)
 constexpr int kEpiWarps = 8;
@@ -239,6 +240,7 @@ enum Mode : int { kGram = 0, kPoly = 1, kNext = 2, kLast = 3 };
 struct GemmParams {
   int M, N, K;
   int tiles_m, tiles_n, per_batch, units, k_blocks, splits;
+  int runs;  // accumulators that a block of K fills (split products of a short K: one for each 16)
   float alpha, beta;
   // kLast: what leaves
   int dtype, step;
@@ -342,6 +344,19 @@ __device__ __forceinline__ void mma_block(uint32_t tmem_d, uint64_t adesc, uint6
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(kStepA), "n"(kStepB)
         : "memory");
   }
+}
+// One MMA (16 of K), by one elected lane.
+template <int CG>
+__device__ __forceinline__ void mma_step(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  static_assert(CG == 1);
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "elect.sync r|e, 0xffffffff;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 // Arrive on `bar` in every CTA of the pair once the MMAs issued so far are complete.
 template <int CG>
@@ -559,10 +574,14 @@ struct Maps {  // high and low parts: operands, addend, result
 };
 
 // SPLIT: a stage holds both parts of both operands, loaded once for the three products of a block of K:
-// low x high and high x low first, then high x high.  The tensor core truncates as it accumulates, which
-// over a long K would cost a few bits of the 22, so every block's sum is added up in fp32 registers
-// (errors after five steps: 1.0e-6 at 1000 x 3000, 2.4e-6 at 600 x 5000, as fp32's own products; 1.3e-5
-// at 1100 x 1030 when each product was one accumulation over K).
+// low x high and high x low first, then high x high.  The tensor core truncates as it accumulates, always
+// towards zero, which over a long K would cost a few bits of the 22, so every block's sum is added up in
+// fp32 registers (errors after five steps: 1.0e-6 at 1000 x 3000, 2.4e-6 at 600 x 5000, as fp32's own
+// products; 1.3e-5 at 1100 x 1030 when each product was one accumulation over K).  A short K has too few
+// sums for fp32's own roundings to be worse than a block's four truncations, so there every 16 of K
+// have an accumulator (63 x 1317: 1.7e-6, by blocks of 64 3.5e-6, fp32's own 1.5e-6; 54 x 297 1.4e-6,
+// 2.5e-6 and 1.6e-6; 94 us and 98, nine of 65 x 2810 184 us and 175), which a long K would pay for and
+// not need (1600 x 6400: 1.31 ms, by blocks 1.04 ms, and 1.0e-6 either way).
 // KS (CG = 1): the blocks of K are shared by a cluster of `splits` CTAs, which sum their accumulators over
 // distributed shared memory and finish a share of the tile each.
 template <int CG, int BN, bool KS, bool SPLIT, bool A_MN, bool B_MN, int MODE>
@@ -572,7 +591,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   constexpr int R = CG * BM / BN;     // a tile is R times as high as wide
   constexpr int kCols = BN / CG;      // columns of the tile whose operand rows this CTA loads
   constexpr int kOperandB = kCols * BK * 2;
-  constexpr int kTmemCols = 2 * BN;
+  constexpr int kAcc = SPLIT ? 4 : 2;  // accumulators in TMEM
+  constexpr int kTmemCols = kAcc * BN;
   constexpr int kParts = SPLIT ? 2 : 1;
   constexpr int kStage = kParts * (kOperand + kOperandB);
   constexpr int kSums = KS ? BN / 32 * 4 * kPartBytes : 0;
@@ -587,11 +607,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   uint64_t* full_bar = bars;
   uint64_t* empty_bar = bars + kSt;
   uint64_t* tfull_bar = bars + 2 * kSt;
-  uint64_t* tempty_bar = bars + 2 * kSt + 2;
-  uint64_t* drain_bar = bars + 2 * kSt + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kSt + 5);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * kSt + 6);
-  uint64_t* c_bar = bars + 2 * kSt + 7;  // two per epilogue warp
+  uint64_t* tempty_bar = tfull_bar + kAcc;
+  uint64_t* drain_bar = tempty_bar + kAcc;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain_bar + 2);
+  uint64_t* c_bar = drain_bar + 3;  // two per epilogue warp
+  static_assert((2 * kSt + 2 * kAcc + 3 + 2 * kEpiWarps) * 8 <= 512);
 
   // (Through a shuffle: the compiler then knows that a warp's role is the same for all its lanes, and
   // keeps the issuing loops' addresses and descriptors in uniform registers.)
@@ -607,7 +628,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < kAcc; ++a) {
       mbar_init(&tfull_bar[a], 1);
       mbar_init(&tempty_bar[a], CG * kEpiWarps);
     }
@@ -724,13 +745,41 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           const bool once = same(tm, tn);
           const uint64_t b_st = once ? a_st + static_cast<uint32_t>((tn % R) * (kOperand / 2) >> 4)
                                      : b_base + static_cast<uint32_t>(stage * kParts * kOperandB >> 4);
+          const uint32_t a_low = static_cast<uint32_t>(kOperand >> 4);
           const uint32_t b_low = static_cast<uint32_t>((once ? kOperand : kOperandB) >> 4);
+          constexpr uint32_t kStepA = A_MN ? 128 : 2, kStepB = B_MN ? 128 : 2;  // 16 of K on
+          bool whole = true;  // the block is one accumulator's
+          if constexpr (SPLIT) whole = p.runs == 1;
+          if (whole) {
 #pragma unroll
-          for (int t = SPLIT ? 0 : 2; t < 3; ++t) {  // low x high, high x low, high x high
-            const uint64_t at = a_st + (t == 0 ? static_cast<uint32_t>(kOperand >> 4) : 0u);
-            const uint64_t bt = b_st + (t == 1 ? b_low : 0u);
-            mma_block<CG, A_MN ? 128 : 2, B_MN ? 128 : 2>(d_tmem, at, bt, idesc,
-                                                          (i > i0 || (SPLIT && t > 0)) ? 1u : 0u);
+            for (int t = SPLIT ? 0 : 2; t < 3; ++t) {  // low x high, high x low, high x high
+              const uint64_t at = a_st + (t == 0 ? a_low : 0u);
+              const uint64_t bt = b_st + (t == 1 ? b_low : 0u);
+              mma_block<CG, kStepA, kStepB>(d_tmem, at, bt, idesc, (i > i0 || (SPLIT && t > 0)) ? 1u : 0u);
+            }
+          }
+          if constexpr (SPLIT) {
+            if (!whole) {  // an accumulator for every 16 of K
+#pragma unroll 1
+              for (int r = 0; r < BK / 16; ++r) {
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                mma_step<CG>(d, a_st + a_low + r * kStepA, b_st + r * kStepB, idesc, 0u);
+                mma_step<CG>(d, a_st + r * kStepA, b_st + b_low + r * kStepB, idesc, 1u);
+                mma_step<CG>(d, a_st + r * kStepA, b_st + r * kStepB, idesc, 1u);
+                if (r + 1 == BK / 16) break;  // (handed over below)
+                commit_all<CG>(&tfull_bar[acc]);
+                if (++acc == kAcc) {
+                  acc = 0;
+                  acc_phase ^= 1u;
+                }
+                if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.status, 422, abort_flag)) {
+                  ok = false;
+                  break;
+                }
+                tc_fence_after();
+              }
+              if (!ok) break;
+            }
           }
           commit_all<CG>(&empty_bar[stage]);
           if (++stage == kSt) {
@@ -740,7 +789,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         if (!ok) break;
         commit_all<CG>(&tfull_bar[acc]);
-        if (++acc == 2) {
+        if (++acc == kAcc) {
           acc = 0;
           acc_phase ^= 1u;
         }
@@ -755,8 +804,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     constexpr int kChunks = BN / 64;       // 32-column chunks per warp
     int acc = 0;
     uint32_t acc_phase = 0;
-    uint32_t tempty[2] = {smem_u32(&tempty_bar[0]), smem_u32(&tempty_bar[1])};
+    uint32_t tempty[2] = {smem_u32(&tempty_bar[0]), smem_u32(&tempty_bar[1])};  // (CG = 2: the leader's)
     if constexpr (CG == 2) {
+      static_assert(kAcc == 2);
       tempty[0] = map_to_cta(tempty[0], 0);
       tempty[1] = map_to_cta(tempty[1], 0);
     }
@@ -769,7 +819,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         else
           mbar_arrive(&tempty_bar[acc]);
       }
-      if (++acc == 2) {
+      if (++acc == kAcc) {
         acc = 0;
         acc_phase ^= 1u;
       }
@@ -829,7 +879,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     auto add_runs = [&](float (&sum)[kChunks * 32]) {
 #pragma unroll
       for (int j = 0; j < kChunks * 32; ++j) sum[j] = 0.f;
-      for (int i0 = lo; i0 < hi; i0 += run) {
+      for (int r = (hi - lo) * p.runs; r > 0; --r) {
         if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) {
           ok = false;
           return;
@@ -1084,6 +1134,7 @@ cudaError_t launch_product(const Pair& a, const Pair& b, const Pair& c, const Pa
   p.per_batch = static_cast<int>(tiles_of(SYM, p.M, p.N, BM * CG, BN));
   p.units = p.per_batch * count;
   p.k_blocks = (p.K + BK - 1) / BK;
+  p.runs = p.K <= kShort ? BK / 16 : 1;
   auto kern = product_kernel<CG, BN, KS, SPLIT, A_MN, B_MN, MODE>;
   static int done[64] = {0};
   int dev = 0;

@@ -312,6 +312,12 @@ __device__ __forceinline__ void expect_elect(uint64_t* bar, uint32_t bytes) {
       "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(smem_u32(bar)), "r"(bytes)
       : "memory");
 }
+// A bounded wait by a whole warp: its lanes go on, or give up, together, as the elections and barriers that
+// follow need them to.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Status* st, uint32_t where,
+                                          volatile int* abort_flag) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, st, where, abort_flag));
+}
 // The four MMAs of a block of K (their descriptors are a step of 16 of K apart), by one elected lane.
 template <int CG, int kStepA, int kStepB>
 __device__ __forceinline__ void mma_block(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -675,7 +681,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       const int col = tn * BN + static_cast<int>(crank) * kCols;
       for (int i = lo; i < hi; ++i) {
         const int k = i * BK;
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, 420, abort_flag))) {
+        if (!warp_wait(&empty_bar[stage], phase ^ 1u, p.status, 420, abort_flag)) {
           ok = false;
           break;
         }
@@ -722,23 +728,19 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const uint64_t b_base = sdesc_sw128(smem_u32(sB), B_MN ? kHalfTile : 16, 1024);
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
+    // A wait that ran out is noted, and the warp goes on to where it hands its sums over: the lanes stay
+    // together without a vote for every block of K (which cost 3 % at 768 x 768).
     bool ok = true;
     for (int u = first; u < p.units && ok; u += stride) {
       int b, tm, tn;
       decode<SYM, R>(p, u, b, tm, tn);
       for (int i0 = lo; i0 < hi; i0 += run) {
-        if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.status, 422, abort_flag)) {
-          ok = false;
-          break;
-        }
+        ok &= mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.status, 422, abort_flag);
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
         const int i1 = min(hi, i0 + run);
         for (int i = i0; i < i1; ++i) {
-          if (!mbar_wait(&full_bar[stage], phase, p.status, 423, abort_flag)) {
-            ok = false;
-            break;
-          }
+          ok &= mbar_wait(&full_bar[stage], phase, p.status, 423, abort_flag);
           tc_fence_after();
           const uint64_t a_st = a_base + static_cast<uint32_t>(stage * kParts * kOperand >> 4);
           // (64 rows of a stage, in either order, are half an operand on)
@@ -766,19 +768,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 mma_step<CG>(d, a_st + a_low + r * kStepA, b_st + r * kStepB, idesc, 0u);
                 mma_step<CG>(d, a_st + r * kStepA, b_st + b_low + r * kStepB, idesc, 1u);
                 mma_step<CG>(d, a_st + r * kStepA, b_st + r * kStepB, idesc, 1u);
-                if (r + 1 == BK / 16) break;  // (handed over below)
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok || r + 1 == BK / 16) break;  // (handed over below)
                 commit_all<CG>(&tfull_bar[acc]);
                 if (++acc == kAcc) {
                   acc = 0;
                   acc_phase ^= 1u;
                 }
-                if (!mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.status, 422, abort_flag)) {
-                  ok = false;
-                  break;
-                }
+                ok &= mbar_wait(&tempty_bar[acc], acc_phase ^ 1u, p.status, 422, abort_flag);
                 tc_fence_after();
               }
-              if (!ok) break;
             }
           }
           commit_all<CG>(&empty_bar[stage]);
@@ -787,7 +786,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             phase ^= 1u;
           }
         }
-        if (!ok) break;
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;  // (not handed over)
         commit_all<CG>(&tfull_bar[acc]);
         if (++acc == kAcc) {
           acc = 0;
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
       for (int j = 0; j < kChunks * 32; ++j) sum[j] = 0.f;
       for (int r = (hi - lo) * p.runs; r > 0; --r) {
-        if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) {
+        if (!warp_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) {
           ok = false;
           return;
         }
@@ -902,7 +902,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       for (int j = 0; j < 32; ++j) v[j] *= p.alpha;
       if constexpr (kAddend) {
         if (kSlots == 2 && more) fetch(ctr + 1, b, row0, n0 + 32);
-        if (!mbar_wait(&cb[ctr % kSlots], static_cast<uint32_t>(ctr / kSlots) & 1u, p.status, 426, abort_flag)) {
+        if (!warp_wait(&cb[ctr % kSlots], static_cast<uint32_t>(ctr / kSlots) & 1u, p.status, 426, abort_flag)) {
           ok = false;
           return;
         }
@@ -986,7 +986,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
           }
         }
       } else {
-        ok = mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag);
+        ok = warp_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag);
         if (ok) {
           tc_fence_after();
 #pragma unroll 1
@@ -1035,7 +1035,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
               finish(v, b, row0, col0 + c * 32, c + 1 < chunks);
             }
         } else {
-          if (!mbar_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) break;
+          if (!warp_wait(&tfull_bar[acc], acc_phase, p.status, 425, abort_flag)) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < chunks && ok; ++c) {

@@ -19,6 +19,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 # MINIDIST_BOUNDS_CHECK=1 loads the checking build (python -m minidist._build --bounds-check).
 _LIB_PATH = Path(__file__).resolve().parent.parent / "_lib" / (
@@ -223,6 +224,12 @@ _HERE = contextlib.nullcontext()
 def on_device(t: torch.Tensor):
     """Context in which ``t``'s device is current (free when it already is)."""
     return _HERE if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def in_forward_mode() -> bool:
+    """Whether a forward-mode level is open, so that tensors may carry tangents (asked before every
+    call: torch's own test of a tensor costs as much as a check of all arguments)."""
+    return forward_ad._current_level >= 0
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

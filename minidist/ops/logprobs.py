@@ -198,7 +198,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     ids = tokens.contiguous() if tokens.dim() == 1 else tokens.reshape(-1).contiguous()
     # (A forward-mode tangent goes the same way, where torch says that there is no such derivative: a
     # kernel launch by itself would drop it.)
-    need = (logits.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(logits).tangent is not None
+    need = (logits.requires_grad and torch.is_grad_enabled()) \
+        or (nat.in_forward_mode() and forward_ad.unpack_dual(logits).tangent is not None)
     if not logits.is_cuda:
         out = _Lookup.apply(flat, ids, temperature, top, entropy, ignore_index)
     elif need:

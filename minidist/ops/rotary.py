@@ -99,10 +99,11 @@ def _launch(q, k, q_out, k_out, table, positions, interleaved: bool, inverse: bo
         pos, wide, ps = positions.data_ptr(), positions.dtype == torch.int64, positions.stride()
         if len(ps) == 1:
             ps = (0, ps[0])
-    if table.data_ptr() % (8 if table.shape[1] % 2 else 16):  # (a slice of rows starts where the kernel can)
+    half = table.shape[1]
+    if table.data_ptr() % (8 if half % 2 else 16):  # (a slice of rows starts where the kernel can)
         table = table.clone()
     params = _PARAMS.pack(q.data_ptr(), kp, q_out.data_ptr(), kop, *xs, *kxs, *ys, *kys, H, Hk, table.data_ptr(),
-                          table.shape[0], pos, wide, *ps, B, S, D, 2 * table.shape[1], interleaved, inverse,
+                          table.shape[0], pos, wide, *ps, B, S, D, 2 * half, interleaved, inverse,
                           _DTYPE_CODE[q.dtype], nat.status_ptr(q.device))
     with nat.on_device(q):
         nat.check(nat.lib().md_rotary(params, nat.stream_ptr()), "md_rotary")
@@ -154,9 +155,10 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, table, positions, interleaved, inverse):
         ctx.save_for_backward(table, positions)
-        ctx.save_for_forward(table, positions)
         ctx.how = (interleaved, inverse)
-        ctx.shapes = (q.shape, None if k is None else k.shape)
+        if nat.in_forward_mode():
+            ctx.save_for_forward(table, positions)
+            ctx.shapes = (q.shape, None if k is None else k.shape)
         ctx.set_materialize_grads(False)
         return tuple(_turn(q, k, table, positions, interleaved, inverse))
 
@@ -221,8 +223,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, p
     :func:`minidist.ops._native.check_status` (on CPU it raises).
     """
     _check(q, k, table, positions)
-    grad = torch.is_grad_enabled()
-    if (grad and (q.requires_grad or (k is not None and k.requires_grad))) or _has_tangent(q) or _has_tangent(k):
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) \
+            or (nat.in_forward_mode() and (_has_tangent(q) or _has_tangent(k))):
         return _Rotary.apply(q, k, table, positions, interleaved, False)
     return tuple(_turn(q, k, table, positions, interleaved, False))
 

@@ -34,7 +34,7 @@
 // entropy 138 us forward (6.0 TB/s) and 269 us backward (6.1 TB/s); 4096 rows
 // without entropy 72 us (5.7 TB/s), with entropy and 20 alternatives 102 us
 // (4.0 TB/s: the selection's chain of dependent steps, about 2 us a row, is only
-// partly hidden by the other blocks of the SM).  fp32, 5 alternatives: 5.6 TB/s.
+// partly hidden by the other blocks of the SM).  fp32, 5 alternatives: 5.5 TB/s.
 // One row of fp32 with 5 alternatives: 8 us, most of it the latency of a cluster's
 // launch, first loads and joins.
 #include <cuda_fp16.h>

@@ -36,7 +36,7 @@
 // power cap), useful operations, symmetric ones counted once: 4096 x 4096, five
 // steps, 1.09 ms = 1260 TFLOP/s in bursts, 1.32 ms = 1040 sustained (tensor pipe
 // active 76 to 82 % of the time; the rest is the last wave of 256 tiles on 74
-// pairs).  12 x 2304 x 768 with momentum and weights 465 us = 585 TFLOP/s: K is 768,
+// pairs).  12 x 2304 x 768 with momentum and weights 470 us = 579 TFLOP/s: K is 768,
 // so a tile brings 512 KB of addend and result to 768 KB of operands (tensor pipe
 // 59 % active in X^T X, 40 % in the update).  768 x 768 89 us: 17 launches of 5.3 us,
 // each a chain of launch, first load, 12 blocks of K (410 cycles each: 60 bytes of
@@ -1201,10 +1201,10 @@ cudaError_t product(int tile, bool split, const Pair& a, const Pair& b, const Pa
   // of K on a pair (512 cycles).  A chain is the first tile's products, then for every further tile the
   // longer of its products and its epilogue, then the last epilogue; a small tile has half the products
   // and epilogue at 0.8 and 0.57 of the time (its operands are loaded 1.5 times as often), a pair 5
-  // blocks more to begin and end.  The constants are fitted to 24 shapes.  One / pairs / the rule, us
-  // for five steps: 12 x 768 x 768 200 / 222 / 200, 4 x 1024 x 1024 158 / 208 / 155, 12 x 2304 x 768
-  // 433 / 424 / 410, 1600 x 6400 420 / 436 / 370, 2500 x 2500 699 / 486 / 494, 4096 x 4096 1308 / 1106 /
-  // 1083; it errs by 3 % at 24 x 768 x 768 (377 / 349 / 366).
+  // blocks more to begin and end.  The constants are fitted to 24 shapes (profiles/operators.md).  One /
+  // pairs / the rule, us for five steps: 12 x 768 x 768 199 / 223 / 200, 4 x 1024 x 1024 165 / 223 / 151,
+  // 12 x 2304 x 768 434 / 425 / 419, 1600 x 6400 408 / 467 / 362, 2500 x 2500 711 / 485 / 485, 4096 x 4096
+  // 1312 / 1119 / 1127; it errs most, by 3 %, at 5 x 1500 x 1700 (649 / 530 / 544).
   auto chain = [](long long waves, float main, float epilogue) {
     return main + static_cast<float>(waves - 1) * fmaxf(main, epilogue) + epilogue;
   };

@@ -22,12 +22,14 @@
 // through are copied by the same threads in vectors of their own width.
 //
 // Measured (B200, copy rate 6.55 TB/s): 20011 tokens of 32 + 32 heads of 80, 40 of
-// them turned, bf16: 74 us, 5.5 TB/s (a loop over vectors with divisions and single
+// them turned, bf16: 76 us, 5.4 TB/s (a loop over vectors with divisions and single
 // conversions: 190 us, of which 45 % was issuing instructions); 16 x 1024 tokens of
 // 12 + 12 heads of 64 in a packed projection: 20 us, 5.0 TB/s, a third of it start
 // and end of so short a launch; fp32 heads of 128: 6.4 TB/s; one token for each of
-// 32 sequences: 1.9 us.  Two heads per thread instead of four measured the same
-// within 5 % on paired layouts and 15 % slower on interleaved ones.
+// 32 sequences: 1.9 us.  An odd R/2 in the half layout, or odd strides, go by single
+// channels: the prompt with 50 of 80 turned 129 us (interleaved, by pairs, 104).
+// Two heads per thread instead of four measured the same within 5 % on paired layouts
+// and 15 % slower on interleaved ones.
 #include <cuda_fp16.h>
 
 #include <type_traits>

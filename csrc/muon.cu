@@ -1020,11 +1020,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         int chunks = 0;  // (those wanted come first)
         while (chunks < kChunks && wanted(row0, col0 + chunks * 32)) ++chunks;
         if (kAddend && chunks > 0) fetch(ctr, b, row0, col0);
-        if constexpr (MODE == kLast)
+        // (Split products of narrow tiles ask for the old weights after their sums: together they spill.)
+        constexpr bool kLate = SPLIT && BN == 64;
+        if constexpr (MODE == kLast && !kLate)
           if (chunks > 0) prepare_out(b, row0, col0);
         if constexpr (SPLIT) {
           float sum[kChunks * 32];
           add_runs(sum);
+          if constexpr (MODE == kLast && kLate)
+            if (chunks > 0) prepare_out(b, row0, col0);
           // (unrolled, so that the sums stay in registers)
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)

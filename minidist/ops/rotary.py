@@ -49,8 +49,11 @@ class RotaryScaling:
     def __post_init__(self):
         if self.kind not in ("linear", "ntk", "yarn"):
             raise ValueError(f"RotaryScaling kind {self.kind!r}: expected 'linear', 'ntk' or 'yarn'")
-        if not self.factor >= 1.0:
-            raise ValueError(f"RotaryScaling factor {self.factor}: expected a value of at least 1")
+        if not 1.0 <= self.factor < math.inf:
+            raise ValueError(f"RotaryScaling factor {self.factor}: expected a finite value of at least 1")
+        if self.original_positions < 1 or not 0.0 < self.beta_slow <= self.beta_fast < math.inf:
+            raise ValueError(f"RotaryScaling original_positions={self.original_positions}, beta_fast={self.beta_fast}, "
+                             f"beta_slow={self.beta_slow}: expected at least one position and 0 < beta_slow <= beta_fast")
 
 
 def rotary_table(rotary_dim: int, positions: int, *, base: float = 10000.0, scaling: RotaryScaling | None = None,

@@ -65,3 +65,13 @@ def test_a_table_that_asks_for_a_gradient_is_refused(device):
             md.apply_rotary(q, None, table)
         with torch.no_grad():
             md.apply_rotary(q, None, table)
+
+
+@pytest.mark.parametrize("bad", [dict(factor=float("inf")), dict(factor=float("nan")), dict(original_positions=0),
+                                 dict(beta_slow=0.0), dict(beta_fast=0.5), dict(beta_fast=float("nan")),
+                                 dict(beta_fast=float("inf"))])
+def test_scaling_refusals(bad):
+    """What would make a table of NaN, of nothing turning, or fail inside it."""
+    with pytest.raises(ValueError, match="RotaryScaling"):
+        md.RotaryScaling("yarn", **{"factor": 2.0, **bad})
+    assert md.rotary_table(16, 8, scaling=md.RotaryScaling("yarn", 2.0, 1, beta_fast=2.0, beta_slow=2.0)).isfinite().all()

@@ -173,10 +173,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     it (entropy and alternatives are computed for every row).  A row without any logit above
     ``-inf`` gives ``-inf``, entropy 0, the lowest tokens as alternatives and no gradient; a NaN or
     ``+inf`` logit makes its row's numbers NaN.  Logits may be a strided view with contiguous rows
-    (the LM head's padded ones; a view whose rows are not equally far apart, such as
-    ``logits[:, :-1]`` of a batch, is copied: shift the tokens and ignore the last one instead); of a tensor-parallel model gather the vocabulary first.  A token
-    outside the vocabulary gives NaN, reported by :func:`minidist.ops._native.check_status` (on CPU
-    it raises).  ``top`` is at most 64.  Differentiable once, in reverse mode.
+    (the LM head's padded ones); one whose rows are not equally far apart, such as
+    ``logits[:, :-1]`` of a batch, is copied (shift the tokens and ignore the last one instead).
+    Of a tensor-parallel model gather the vocabulary first.  A token outside the vocabulary gives
+    NaN, reported by :func:`minidist.ops._native.check_status` (on CPU it raises).  ``top`` is at
+    most 64.  Differentiable once, in reverse mode.
     """
     if logits.dim() < 1 or logits.dtype not in _DTYPE_CODE:
         raise TypeError(f"token_logprobs: logits {tuple(logits.shape)} {logits.dtype} are not bfloat16, float16 or "

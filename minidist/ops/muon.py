@@ -157,10 +157,10 @@ def orthogonalize(u: torch.Tensor, *, steps: int = 5, coefficients: Sequence[flo
 
     The polynomial ``a s + b s^3 + c s^5`` has to keep ``|s| <= 1.3`` within about two, as the default
     and the classical ``(1.5, -0.5, 0)`` and ``(15/8, -10/8, 3/8)`` do; one that could leave the range of
-    the kernels' operands (``s^2`` or ``b s^2 + c s^4`` of 15.5) is refused on CUDA.  bfloat16 results are within a
-    bfloat16 rounding or so of exact, float16 and float32 ones within their own type's; ``precise``
-    takes those types' products (three of fp16 parts each instead of one) for bfloat16 as well, whose
-    results are then off by their rounding alone.  Not differentiable."""
+    the kernels' operands (``s^2`` or ``b s^2 + c s^4`` of 15.5) is refused on CUDA.  bfloat16 results
+    are within a bfloat16 rounding or so of exact, float16 and float32 ones within their own type's;
+    ``precise`` takes those types' products (three of fp16 parts each instead of one) for bfloat16 as
+    well, whose results are then off by their rounding alone.  Not differentiable."""
     if u.dim() < 2 or u.dtype not in _DTYPE_CODE:
         raise TypeError(f"orthogonalize: {tuple(u.shape)} {u.dtype} is not a bfloat16, float16 or float32 matrix")
     _check_polynomial(steps, coefficients, eps)
